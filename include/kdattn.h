@@ -213,13 +213,121 @@ typedef struct kd_x3_args {
   int32_t pad_;
 } kd_x3_args;
 
+/* Eight-bit blocks (kd_quant_rows8 .. kd_weight_grad8): values in OCP e4m3 with
+ * one scale 2^e a block of 128 consecutive columns of a row, or of 128 x 128
+ * values of a weight; e is the least integer with max |x| <= 448 2^e over the
+ * block's finite values, stored as the byte e + 127 (e8m0; 127 for a block of
+ * zeros).  Values that are not finite become NaN.  Rows of e4m3 lie y_stride
+ * bytes apart, a multiple of 16 and at least the columns rounded up to 16, whose
+ * last 8 bytes are written as zeros where the columns are no multiple of 16.
+ * scale is [rows, ceil(columns / 128)], contiguous. */
+typedef struct {
+  const void *x[4];         /* n parts side by side: [rows, cols[i]], all but the last a multiple of 128 wide */
+  int64_t x_stride[4];      /* rows apart, in elements, a multiple of 8 */
+  int32_t cols[4];          /* multiples of 8 */
+  int32_t n, dtype;         /* 1 .. 4; bf16, fp16 or fp32 */
+  int64_t rows;
+  uint8_t *y;
+  int64_t y_stride;
+  uint8_t *scale;
+  int32_t total, pad_;      /* sum of cols */
+} kd_rows8_args;
+
+typedef struct {
+  const void *w[4];         /* n parts one below the other: [rows[i], K], all but the last a multiple of 128 high */
+  int64_t w_stride[4];
+  int32_t rows[4];
+  int32_t n, dtype;
+  int32_t K, total;         /* K a multiple of 8; total: sum of rows, a multiple of 8 where yt is given */
+  uint8_t *y;               /* [total, K] */
+  int64_t y_stride;
+  uint8_t *scale;           /* [ceil(total / 128), ceil(K / 128)] */
+  uint8_t *yt;              /* [K, total], or NULL */
+  int64_t yt_stride;
+  uint8_t *scale_t;         /* [ceil(K / 128), ceil(total / 128)], or NULL */
+} kd_weight8_args;
+
+typedef struct {
+  const uint8_t *a;         /* [M, K] e4m3, rows lda bytes apart (a multiple of 16) */
+  const uint8_t *b;         /* [N, K] */
+  int64_t lda, ldb;
+  const uint8_t *a_scale;   /* [M, ceil(K / 128)] */
+  const uint8_t *b_scale;   /* [ceil(N / 128), ceil(K / 128)] */
+  void *out;                /* [M, N], rows ldo elements apart */
+  int64_t ldo;
+  int32_t M, N, K, dtype;   /* K a multiple of 16; the type of out */
+} kd_matmul8_args;
+
+typedef struct {
+  const void *x, *delta;    /* [rows, D] contiguous bf16 / fp16; delta NULL: nothing is added */
+  void *sum;                /* [rows, D], x + delta rounded (with delta) */
+  uint8_t *y;
+  int64_t y_stride;
+  uint8_t *scale;
+  float *rstd;              /* [rows], or NULL */
+  int64_t rows;
+  int32_t D, dtype;         /* D a multiple of 8 in 8 .. 8192 */
+  float eps;
+  int32_t pad_;
+} kd_norm8_args;
+
+typedef struct {
+  const void *g, *ds;       /* gradients of y and of sum (NULL: none), [rows, D] contiguous */
+  const uint8_t *y;
+  int64_t y_stride;
+  const uint8_t *scale;
+  const float *rstd;
+  void *dx;                 /* the gradient of x, and of delta */
+  int64_t rows;
+  int32_t D, dtype;
+} kd_norm8_bwd_args;
+
+typedef struct {
+  const void *a, *b;        /* forward: [rows, H] bf16 / fp16 */
+  int64_t a_stride, b_stride;
+  uint8_t *y8, *y_scale;    /* forward: silu(a) b */
+  uint8_t *a8, *a_scale, *b8, *b_scale; /* a and b: written (NULL: not kept), read by the backward */
+  int64_t stride;           /* of all e4m3 rows */
+  const void *dy;           /* backward: [rows, H] contiguous, and the results alike */
+  void *da, *db;
+  int64_t rows;
+  int32_t H, dtype;         /* H a multiple of 8 */
+} kd_gate8_args;
+
+typedef struct {
+  const void *dy;           /* [M, N] bf16 / fp16, rows ldy elements apart (a multiple of 8) */
+  int64_t ldy;
+  const uint8_t *x;         /* [M, K] e4m3, rows ldx bytes apart */
+  int64_t ldx;
+  const uint8_t *x_scale;   /* [M, ceil(K / 128)] */
+  void *dw;                 /* [N, K] contiguous, dy's type */
+  float *ws;                /* kd_weight_grad8_ws_bytes, used by this call alone */
+  int64_t ws_bytes;
+  int32_t M, N, K, dtype;   /* N and K multiples of 8 */
+} kd_wgrad8_args;
+
+typedef struct {
+  const void *tokens;       /* [n] contiguous */
+  int64_t n;
+  const void *weight;       /* [vocab, dim] contiguous bf16, fp16 or fp32 */
+  void *out;                /* [n, dim]: scale * weight[token]; NaN for a token outside 0 .. vocab - 1 */
+  const void *dy;           /* gradient: [n, dim] contiguous */
+  void *dw;                 /* gradient: [vocab, dim], written in full */
+  int64_t vocab, dim;
+  int64_t padding_idx;      /* this token's row of dw stays zero (-1: none) */
+  int32_t tokens_dtype, dtype;
+  float scale;
+  int32_t pad_;
+} kd_embed_args;
+
 /* Library version (major*10000 + minor*100 + patch).  3.0.0: the plan's size
  * beside its pointer in every entry point that takes a plan.  3.1.0:
  * kd_plan_layout writes 20 offsets (the dK/dV work order added).  3.2.0:
  * kd_absmax added.  3.3.0: fp8 scores (q8 / k8) and kd_quant_fp8 at head
  * dim 256.  3.4.0: attention with a workspace (kd_attn_fwd_ws, kd_attn_bwd_ws),
  * kd_signs, kd_span_count, kd_rms_norm, kd_swiglu, kd_weight_grad, kd_x3_pack
- * and kd_x3_unpack added.  3.5.0: kd_attn_args.lists, a padding word before. */
+ * and kd_x3_unpack added.  3.5.0: kd_attn_args.lists, a padding word before.
+ * 3.6.0: 8-bit blocks (kd_quant_rows8 .. kd_weight_grad8) and kd_embed added. */
 int kd_version(void);
 
 /* Message for the last non-zero status returned on this thread. */
@@ -367,6 +475,38 @@ int kd_swiglu_bwd(const void *a, const void *b, const void *dy, void *da, void *
 int64_t kd_weight_grad_ws_bytes(int32_t M, int32_t N, int32_t K, int32_t dtype);
 int kd_weight_grad(const void *dy, const void *x, void *dw, int32_t M, int32_t N, int32_t K, int32_t dtype,
                    void *ws, int64_t ws_bytes, void *stream);
+
+/* Rows, and a weight (with its transpose for products over its rows), to 8-bit blocks. */
+int kd_quant_rows8(const kd_rows8_args *a, void *stream);
+int kd_quant_weight8(const kd_weight8_args *a, void *stream);
+
+/* out = A B^T of 8-bit blocks, fp32 sums, rounded once to out's type. */
+int kd_matmul8(const kd_matmul8_args *a, void *stream);
+
+/* sum = x + delta, rounded; y = sum rsqrt(mean(sum^2) + eps) in 8-bit blocks
+ * (model.py:31-39 after the residual's addition); and dx = ds + rstd (g - y
+ * mean(g y)) from the 8-bit y. */
+int kd_norm8(const kd_norm8_args *a, void *stream);
+int kd_norm8_bwd(const kd_norm8_bwd_args *a, void *stream);
+
+/* y = silu(a) b in 8-bit blocks (model.py:42-52), a and b kept in 8-bit blocks,
+ * and the gradients of a and b from those. */
+int kd_gate8(const kd_gate8_args *a, void *stream);
+int kd_gate8_bwd(const kd_gate8_args *a, void *stream);
+
+/* dW [N, K] = dY^T X with X in 8-bit blocks, fp32 sums, rounded once. */
+int64_t kd_weight_grad8_ws_bytes(int32_t M, int32_t N, int32_t K, int32_t dtype);
+int kd_weight_grad8(const kd_wgrad8_args *a, void *stream);
+
+/* Embedding lookup (model.py:127-178) and its gradient, the sums in fp32 in the
+ * order of the positions, without atomics.  ws: kd_embed_grad_ws_bytes, 16-byte
+ * aligned, used by this call alone. */
+int kd_embed(const kd_embed_args *a, void *stream);
+int64_t kd_embed_grad_ws_bytes(int64_t n, int64_t vocab, int64_t dim);
+int kd_embed_grad(const kd_embed_args *a, void *ws, int64_t ws_bytes, void *stream);
+
+/* sizeof the structs of the above, in the order they are declared: 8 values */
+void kd_struct_sizes6(size_t *sizes);
 
 /* fp32 rows x as packed bf16 rows of h = bf16(x) and l = bf16(x - h), zeros
  * behind (pack), and the fp32 sum of a packed result's blocks 0 and sel, each with

@@ -119,6 +119,86 @@ class X3Args(ctypes.Structure):
     ]
 
 
+class Rows8Args(ctypes.Structure):
+    """Mirror of ``kd_rows8_args``."""
+
+    _fields_ = [
+        ("x", c_void_p * 4), ("x_stride", c_int64 * 4), ("cols", c_int32 * 4), ("n", c_int32), ("dtype", c_int32),
+        ("rows", c_int64), ("y", c_void_p), ("y_stride", c_int64), ("scale", c_void_p), ("total", c_int32),
+        ("pad_", c_int32),
+    ]
+
+
+class Weight8Args(ctypes.Structure):
+    """Mirror of ``kd_weight8_args``."""
+
+    _fields_ = [
+        ("w", c_void_p * 4), ("w_stride", c_int64 * 4), ("rows", c_int32 * 4), ("n", c_int32), ("dtype", c_int32),
+        ("K", c_int32), ("total", c_int32), ("y", c_void_p), ("y_stride", c_int64), ("scale", c_void_p),
+        ("yt", c_void_p), ("yt_stride", c_int64), ("scale_t", c_void_p),
+    ]
+
+
+class Matmul8Args(ctypes.Structure):
+    """Mirror of ``kd_matmul8_args``."""
+
+    _fields_ = [
+        ("a", c_void_p), ("b", c_void_p), ("lda", c_int64), ("ldb", c_int64), ("a_scale", c_void_p), ("b_scale", c_void_p),
+        ("out", c_void_p), ("ldo", c_int64), ("M", c_int32), ("N", c_int32), ("K", c_int32), ("dtype", c_int32),
+    ]
+
+
+class Norm8Args(ctypes.Structure):
+    """Mirror of ``kd_norm8_args``."""
+
+    _fields_ = [
+        ("x", c_void_p), ("delta", c_void_p), ("sum", c_void_p), ("y", c_void_p), ("y_stride", c_int64),
+        ("scale", c_void_p), ("rstd", c_void_p), ("rows", c_int64), ("D", c_int32), ("dtype", c_int32), ("eps", c_float),
+        ("pad_", c_int32),
+    ]
+
+
+class Norm8BwdArgs(ctypes.Structure):
+    """Mirror of ``kd_norm8_bwd_args``."""
+
+    _fields_ = [
+        ("g", c_void_p), ("ds", c_void_p), ("y", c_void_p), ("y_stride", c_int64), ("scale", c_void_p),
+        ("rstd", c_void_p), ("dx", c_void_p), ("rows", c_int64), ("D", c_int32), ("dtype", c_int32),
+    ]
+
+
+class Gate8Args(ctypes.Structure):
+    """Mirror of ``kd_gate8_args``."""
+
+    _fields_ = [
+        ("a", c_void_p), ("b", c_void_p), ("a_stride", c_int64), ("b_stride", c_int64), ("y8", c_void_p),
+        ("y_scale", c_void_p), ("a8", c_void_p), ("a_scale", c_void_p), ("b8", c_void_p), ("b_scale", c_void_p),
+        ("stride", c_int64), ("dy", c_void_p), ("da", c_void_p), ("db", c_void_p), ("rows", c_int64), ("H", c_int32),
+        ("dtype", c_int32),
+    ]
+
+
+class Wgrad8Args(ctypes.Structure):
+    """Mirror of ``kd_wgrad8_args``."""
+
+    _fields_ = [
+        ("dy", c_void_p), ("ldy", c_int64), ("x", c_void_p), ("ldx", c_int64), ("x_scale", c_void_p), ("dw", c_void_p),
+        ("ws", c_void_p), ("ws_bytes", c_int64), ("M", c_int32), ("N", c_int32), ("K", c_int32), ("dtype", c_int32),
+    ]
+
+
+class EmbedArgs(ctypes.Structure):
+    """Mirror of ``kd_embed_args``."""
+
+    _fields_ = [
+        ("tokens", c_void_p), ("n", c_int64), ("weight", c_void_p), ("out", c_void_p), ("dy", c_void_p), ("dw", c_void_p),
+        ("vocab", c_int64), ("dim", c_int64), ("padding_idx", c_int64), ("tokens_dtype", c_int32), ("dtype", c_int32),
+        ("scale", c_float), ("pad_", c_int32),
+    ]
+
+
+BLOCK8_STRUCTS = (Rows8Args, Weight8Args, Matmul8Args, Norm8Args, Norm8BwdArgs, Gate8Args, Wgrad8Args, EmbedArgs)
+
 # name -> (restype, argtypes); every symbol include/kdattn.h declares
 SIGNATURES = {
     "kd_version": (c_int, []),
@@ -135,6 +215,19 @@ SIGNATURES = {
     "kd_weight_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64,
                                c_void_p]),
     "kd_struct_sizes5": (None, [POINTER(c_size_t)]),
+    "kd_struct_sizes6": (None, [POINTER(c_size_t)]),
+    "kd_quant_rows8": (c_int, [POINTER(Rows8Args), c_void_p]),
+    "kd_quant_weight8": (c_int, [POINTER(Weight8Args), c_void_p]),
+    "kd_matmul8": (c_int, [POINTER(Matmul8Args), c_void_p]),
+    "kd_norm8": (c_int, [POINTER(Norm8Args), c_void_p]),
+    "kd_norm8_bwd": (c_int, [POINTER(Norm8BwdArgs), c_void_p]),
+    "kd_gate8": (c_int, [POINTER(Gate8Args), c_void_p]),
+    "kd_gate8_bwd": (c_int, [POINTER(Gate8Args), c_void_p]),
+    "kd_weight_grad8_ws_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "kd_weight_grad8": (c_int, [POINTER(Wgrad8Args), c_void_p]),
+    "kd_embed": (c_int, [POINTER(EmbedArgs), c_void_p]),
+    "kd_embed_grad_ws_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "kd_embed_grad": (c_int, [POINTER(EmbedArgs), c_void_p, c_int64, c_void_p]),
     "kd_x3_pack": (c_int, [POINTER(X3Args), c_void_p]),
     "kd_x3_unpack": (c_int, [POINTER(X3Args), c_void_p]),
     "kd_rms_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_float, c_void_p]),
@@ -204,6 +297,11 @@ def load():
             f"attn={ctypes.sizeof(AttnArgs)} rot={ctypes.sizeof(RotArgs)} quant={ctypes.sizeof(QuantArgs)} "
             f"tokens={ctypes.sizeof(TokenArgs)} span={ctypes.sizeof(SpanArgs)} "
             f"x3={ctypes.sizeof(X3Args)}")
+    sizes = (c_size_t * len(BLOCK8_STRUCTS))()
+    lib.kd_struct_sizes6(sizes)
+    for got, mirror in zip(sizes, BLOCK8_STRUCTS):
+        if got != ctypes.sizeof(mirror):
+            raise ImportError(f"struct layout mismatch: {mirror.__name__} is {got} bytes in C, {ctypes.sizeof(mirror)} here")
     _lib = lib
     return lib
 

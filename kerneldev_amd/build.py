@@ -66,7 +66,7 @@ def build_library(verbose: bool = False) -> str:
     return LIB
 
 
-NATIVE_SRC = os.path.join(CSRC, "kd_torch.cpp")
+NATIVE_SRCS = [os.path.join(CSRC, f) for f in ("kd_torch.cpp", "kd_torch_block8.cpp")]
 NATIVE = os.path.join(PKG, "_kd_torch.so")
 
 
@@ -81,10 +81,14 @@ def build_native(verbose: bool = False) -> str:
     inc = [f"-I{p}" for p in (*cpp_extension.include_paths(), f"{rocm}/include", sysconfig.get_paths()["include"])]
     libdirs = [f"-L{p}" for p in cpp_extension.library_paths()]
     tmp = NATIVE + ".tmp"
-    _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_kd_torch", *inc, NATIVE_SRC, "-o", tmp,
-          f"-L{PKG}", "-lkdattn", *libdirs, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-          "-Wl,-rpath,$ORIGIN"])
+    os.makedirs(BUILD, exist_ok=True)
+    objs = [os.path.join(BUILD, os.path.basename(src)[:-4] + ".host.o") for src in NATIVE_SRCS]
+    flags = ["-std=c++17", "-O2", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-DTORCH_EXTENSION_NAME=_kd_torch", *inc]
+    with ThreadPoolExecutor(max_workers=len(objs)) as ex:
+        list(ex.map(lambda so: _run(["g++", *flags, "-c", so[0], "-o", so[1]]), zip(NATIVE_SRCS, objs)))
+    _run(["g++", "-shared", *objs, "-o", tmp, f"-L{PKG}", "-lkdattn", *libdirs, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+          "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, NATIVE)
     if verbose:
         print(f"built {NATIVE}")

@@ -119,7 +119,7 @@ int check_plan(const void* plan, int64_t plan_bytes, int B, int T, int D) {
 
 extern "C" {
 
-int kd_version(void) { return 30500; }
+int kd_version(void) { return 30600; }
 
 const char* kd_last_error_string(void) { return g_err.c_str(); }
 
@@ -233,6 +233,208 @@ int kd_weight_grad(const void* dy, const void* x, void* dw, int32_t M, int32_t N
   if (ws_bytes < kd_weight_grad_ws_bytes(M, N, K, dtype)) return fail(KD_ERR_INVALID, "ws is too small");
   r = kd::launch_wgrad(dy, x, dw, static_cast<float*>(ws), M, N, K, dtype, as_stream(stream));
   return r ? fail(r, "kernel launch failed (weight gradient)") : KD_OK;
+}
+
+// ---- 8-bit blocks ---------------------------------------------------------
+static bool type16(int32_t t) { return t == KD_BF16 || t == KD_F16; }
+static int64_t up(int64_t n, int64_t of) { return (n + of - 1) / of * of; }
+// e4m3 rows: base and stride in 16-byte words, the stride at least `cols` rounded up
+static int check_rows8(const void* y, int64_t stride, int64_t cols) {
+  if (y == nullptr || !aligned16(y)) return fail(KD_ERR_INVALID, "e4m3 rows must be given and 16-byte aligned");
+  if (stride % 16 != 0 || stride < up(cols, 16) || stride > (int64_t(1) << 23))
+    return fail(KD_ERR_INVALID, "e4m3 rows must be a multiple of 16 bytes apart, hold their columns and be <= 2^23 bytes apart");
+  return KD_OK;
+}
+static int check_source(const void* x, int64_t stride, int64_t cols) {
+  if (x == nullptr || !aligned16(x)) return fail(KD_ERR_INVALID, "operands must be given and 16-byte aligned");
+  if (stride < cols || stride % 8 != 0) return fail(KD_ERR_INVALID, "rows must be a multiple of 8 elements apart and not overlap");
+  return KD_OK;
+}
+static int check_count(int64_t rows, int64_t cols) {
+  if (rows < 1 || rows > (int64_t(1) << 32)) return fail(KD_ERR_INVALID, "rows must be in 1 .. 2^32");
+  if (cols < 8 || cols % 8 != 0 || cols > (1 << 22)) return fail(KD_ERR_UNSUPPORTED, "columns must be a multiple of 8 in 8 .. 2^22");
+  return KD_OK;
+}
+
+int kd_quant_rows8(const kd_rows8_args* a, void* stream) {
+  int r;
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if (a->n < 1 || a->n > 4) return fail(KD_ERR_INVALID, "n must be in 1 .. 4");
+  if (!type16(a->dtype) && a->dtype != KD_F32) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16, fp16 or fp32");
+  int64_t total = 0;
+  for (int i = 0; i < a->n; ++i) {
+    if ((r = check_count(a->rows, a->cols[i])) || (r = check_source(a->x[i], a->x_stride[i], a->cols[i]))) return r;
+    if (i + 1 < a->n && a->cols[i] % 128 != 0) return fail(KD_ERR_INVALID, "parts before the last must be whole blocks");
+    total += a->cols[i];
+  }
+  if (total != a->total) return fail(KD_ERR_INVALID, "total must be the sum of cols");
+  if ((r = check_count(a->rows, total)) || (r = check_rows8(a->y, a->y_stride, total))) return r;
+  if (a->scale == nullptr) return fail(KD_ERR_INVALID, "scale is required");
+  r = kd::launch_quant_rows(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (rows to 8 bits)") : KD_OK;
+}
+
+int kd_quant_weight8(const kd_weight8_args* a, void* stream) {
+  int r;
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if (a->n < 1 || a->n > 4) return fail(KD_ERR_INVALID, "n must be in 1 .. 4");
+  if (!type16(a->dtype) && a->dtype != KD_F32) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16, fp16 or fp32");
+  int64_t total = 0;
+  for (int i = 0; i < a->n; ++i) {
+    if (a->rows[i] < 1) return fail(KD_ERR_INVALID, "rows must be >= 1");
+    if ((r = check_count(a->rows[i], a->K)) || (r = check_source(a->w[i], a->w_stride[i], a->K))) return r;
+    if (i + 1 < a->n && a->rows[i] % 128 != 0) return fail(KD_ERR_INVALID, "parts before the last must be whole blocks");
+    total += a->rows[i];
+  }
+  if (total != a->total) return fail(KD_ERR_INVALID, "total must be the sum of rows");
+  if (up(total, 128) / 128 * (up(a->K, 128) / 128) >= (1 << 24)) return fail(KD_ERR_UNSUPPORTED, "too many blocks");
+  if ((r = check_rows8(a->y, a->y_stride, a->K))) return r;
+  if (a->scale == nullptr || (a->yt == nullptr) != (a->scale_t == nullptr))
+    return fail(KD_ERR_INVALID, "scale is required, and yt and scale_t go together");
+  if (a->yt != nullptr) {
+    if (total % 8 != 0) return fail(KD_ERR_UNSUPPORTED, "the transpose takes a multiple of 8 rows");
+    if ((r = check_rows8(a->yt, a->yt_stride, total))) return r;
+  }
+  r = kd::launch_quant_weight(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (weight to 8 bits)") : KD_OK;
+}
+
+int kd_matmul8(const kd_matmul8_args* a, void* stream) {
+  int r;
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if (a->M < 1 || a->N < 1) return fail(KD_ERR_INVALID, "M and N must be >= 1");
+  if (a->K < 16 || a->K % 16 != 0 || a->K > (1 << 22)) return fail(KD_ERR_UNSUPPORTED, "K must be a multiple of 16 in 16 .. 2^22");
+  if (!type16(a->dtype) && a->dtype != KD_F32) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16, fp16 or fp32");
+  if ((r = check_rows8(a->a, a->lda, a->K)) || (r = check_rows8(a->b, a->ldb, a->K))) return r;
+  if (a->a_scale == nullptr || a->b_scale == nullptr) return fail(KD_ERR_INVALID, "a_scale and b_scale are required");
+  if (a->out == nullptr || !aligned16(a->out) || a->ldo < a->N) return fail(KD_ERR_INVALID, "out must be given, 16-byte aligned, its rows N apart or more");
+  if (up(a->M, 128) / 128 * (up(a->N, 128) / 128) >= (1 << 24)) return fail(KD_ERR_UNSUPPORTED, "M * N exceeds the grid limit");
+  r = kd::launch_matmul8(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (8-bit product)") : KD_OK;
+}
+
+static int check_norm8(int64_t rows, int32_t D, int32_t dtype) {
+  if (rows < 1 || rows > (int64_t(1) << 32)) return fail(KD_ERR_INVALID, "rows must be in 1 .. 2^32");
+  if (D < 8 || D > 8192 || D % 8 != 0) return fail(KD_ERR_UNSUPPORTED, "D must be a multiple of 8 in 8 .. 8192");
+  if (!type16(dtype)) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16 or fp16");
+  return KD_OK;
+}
+
+int kd_norm8(const kd_norm8_args* a, void* stream) {
+  int r;
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if ((r = check_norm8(a->rows, a->D, a->dtype)) || (r = check_flat({a->x}))) return r;
+  if (a->delta != nullptr && (r = check_flat({a->delta, a->sum}))) return r;
+  if ((r = check_rows8(a->y, a->y_stride, a->D))) return r;
+  if (a->scale == nullptr) return fail(KD_ERR_INVALID, "scale is required");
+  r = kd::launch_norm8(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (norm to 8 bits)") : KD_OK;
+}
+
+int kd_norm8_bwd(const kd_norm8_bwd_args* a, void* stream) {
+  int r;
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if ((r = check_norm8(a->rows, a->D, a->dtype)) || (r = check_flat({a->g, a->dx}))) return r;
+  if (a->ds != nullptr && (r = check_flat({a->ds}))) return r;
+  if ((r = check_rows8(a->y, a->y_stride, a->D))) return r;
+  if (a->scale == nullptr || a->rstd == nullptr) return fail(KD_ERR_INVALID, "scale and rstd are required");
+  r = kd::launch_norm8_bwd(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (norm from 8 bits, backward)") : KD_OK;
+}
+
+static int check_gate8(const kd_gate8_args* a, bool kept) {
+  int r;
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if (!type16(a->dtype)) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16 or fp16");
+  if ((r = check_count(a->rows, a->H))) return r;
+  if (!kept) return KD_OK;
+  if ((r = check_rows8(a->a8, a->stride, a->H)) || (r = check_rows8(a->b8, a->stride, a->H))) return r;
+  if (a->a_scale == nullptr || a->b_scale == nullptr) return fail(KD_ERR_INVALID, "a_scale and b_scale are required");
+  return KD_OK;
+}
+
+int kd_gate8(const kd_gate8_args* a, void* stream) {
+  int r;
+  if ((r = check_gate8(a, a != nullptr && a->a8 != nullptr))) return r;
+  if ((r = check_source(a->a, a->a_stride, a->H)) || (r = check_source(a->b, a->b_stride, a->H))) return r;
+  if ((r = check_rows8(a->y8, a->stride, a->H))) return r;
+  if (a->y_scale == nullptr) return fail(KD_ERR_INVALID, "y_scale is required");
+  r = kd::launch_gate8(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (gate to 8 bits)") : KD_OK;
+}
+
+int kd_gate8_bwd(const kd_gate8_args* a, void* stream) {
+  int r;
+  if ((r = check_gate8(a, true)) || (r = check_flat({a->dy, a->da, a->db}))) return r;
+  r = kd::launch_gate8_bwd(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (gate from 8 bits, backward)") : KD_OK;
+}
+
+static int check_wgrad8(int32_t M, int32_t N, int32_t K, int32_t dtype) {
+  if (M < 1 || N < 8 || K < 8) return fail(KD_ERR_INVALID, "M must be >= 1, N and K >= 8");
+  if (N % 8 != 0 || K % 8 != 0) return fail(KD_ERR_UNSUPPORTED, "N and K must be multiples of 8");
+  if (N > (1 << 22) || K > (1 << 22) || int64_t(N) * K >= (int64_t(1) << 30))
+    return fail(KD_ERR_UNSUPPORTED, "N and K must be <= 2^22 and dW < 2^30 elements");
+  if (!type16(dtype)) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16 or fp16");
+  return KD_OK;
+}
+
+int64_t kd_weight_grad8_ws_bytes(int32_t M, int32_t N, int32_t K, int32_t dtype) {
+  return check_wgrad8(M, N, K, dtype) ? -1 : kd::wgrad8_ws_bytes(M, N, K);
+}
+
+int kd_weight_grad8(const kd_wgrad8_args* a, void* stream) {
+  int r;
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if ((r = check_wgrad8(a->M, a->N, a->K, a->dtype)) || (r = check_flat({a->dw, a->ws}))) return r;
+  if ((r = check_source(a->dy, a->ldy, a->N)) || (r = check_rows8(a->x, a->ldx, a->K))) return r;
+  if (a->ldy > (1 << 23)) return fail(KD_ERR_UNSUPPORTED, "dy's rows must be <= 2^23 elements apart");
+  if (a->x_scale == nullptr) return fail(KD_ERR_INVALID, "x_scale is required");
+  if (a->ws_bytes < kd::wgrad8_ws_bytes(a->M, a->N, a->K)) return fail(KD_ERR_INVALID, "ws is too small");
+  r = kd::launch_wgrad8(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (weight gradient from 8 bits)") : KD_OK;
+}
+
+// ---- embedding --------------------------------------------------------------
+static int check_embed(const kd_embed_args* a) {
+  if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
+  if (a->n < 1 || a->n >= (int64_t(1) << 31)) return fail(KD_ERR_UNSUPPORTED, "n must be in 1 .. 2^31 - 1");
+  if (a->vocab < 1 || a->vocab >= (int64_t(1) << 31) - 1) return fail(KD_ERR_UNSUPPORTED, "vocab must be in 1 .. 2^31 - 2");
+  if (a->dim < 1 || a->dim > (1 << 20)) return fail(KD_ERR_UNSUPPORTED, "dim must be in 1 .. 2^20");
+  if (a->tokens == nullptr) return fail(KD_ERR_INVALID, "tokens is required");
+  if (a->tokens_dtype != KD_I64 && a->tokens_dtype != KD_I32) return fail(KD_ERR_INVALID, "bad tokens dtype");
+  if (!type16(a->dtype) && a->dtype != KD_F32) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16, fp16 or fp32");
+  return KD_OK;
+}
+
+int kd_embed(const kd_embed_args* a, void* stream) {
+  int r;
+  if ((r = check_embed(a))) return r;
+  if (a->weight == nullptr || a->out == nullptr) return fail(KD_ERR_INVALID, "weight and out are required");
+  r = kd::launch_embed(*a, as_stream(stream));
+  return r ? fail(r, "kernel launch failed (embedding)") : KD_OK;
+}
+
+int64_t kd_embed_grad_ws_bytes(int64_t n, int64_t vocab, int64_t dim) {
+  if (n < 1 || n >= (int64_t(1) << 31) || vocab < 1 || vocab >= (int64_t(1) << 31) - 1 || dim < 1 || dim > (1 << 20)) return -1;
+  return kd::embed_grad_ws_bytes(n, vocab, dim);
+}
+
+int kd_embed_grad(const kd_embed_args* a, void* ws, int64_t ws_bytes, void* stream) {
+  int r;
+  if ((r = check_embed(a)) || (r = check_flat({a->dw, ws}))) return r;
+  if (a->dy == nullptr) return fail(KD_ERR_INVALID, "dy is required");
+  if (a->n * up(a->dim, 64) / 64 / 32 >= (int64_t(1) << 31) - 1024) return fail(KD_ERR_UNSUPPORTED, "n * dim exceeds the grid limit");
+  if (ws_bytes < kd::embed_grad_ws_bytes(a->n, a->vocab, a->dim)) return fail(KD_ERR_INVALID, "ws is too small");
+  r = kd::launch_embed_grad(*a, static_cast<uint8_t*>(ws), as_stream(stream));
+  return r ? fail(r, "kernel launch failed (embedding gradient)") : KD_OK;
+}
+
+void kd_struct_sizes6(size_t* s) {
+  if (s == nullptr) return;
+  const size_t v[8] = {sizeof(kd_rows8_args),     sizeof(kd_weight8_args), sizeof(kd_matmul8_args), sizeof(kd_norm8_args),
+                       sizeof(kd_norm8_bwd_args), sizeof(kd_gate8_args),   sizeof(kd_wgrad8_args),  sizeof(kd_embed_args)};
+  for (int i = 0; i < 8; ++i) s[i] = v[i];
 }
 
 int kd_swiglu(const void* a, const void* b, void* y, int64_t n, int32_t dtype, void* stream) {

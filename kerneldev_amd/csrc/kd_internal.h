@@ -82,6 +82,18 @@ int launch_rms_bwd(const void* x, const void* dy, const float* rstd, void* dx, i
 int launch_gate_fwd(const void* a, const void* b, void* y, int64_t n, int dtype, hipStream_t st);
 int launch_gate_bwd(const void* a, const void* b, const void* dy, void* da, void* db, int64_t n, int dtype,
                     hipStream_t st);
+int launch_quant_rows(const kd_rows8_args& a, hipStream_t st);
+int launch_quant_weight(const kd_weight8_args& a, hipStream_t st);
+int launch_matmul8(const kd_matmul8_args& a, hipStream_t st);
+int launch_norm8(const kd_norm8_args& a, hipStream_t st);
+int launch_norm8_bwd(const kd_norm8_bwd_args& a, hipStream_t st);
+int launch_gate8(const kd_gate8_args& a, hipStream_t st);
+int launch_gate8_bwd(const kd_gate8_args& a, hipStream_t st);
+int64_t wgrad8_ws_bytes(int M, int N, int K);
+int launch_wgrad8(const kd_wgrad8_args& a, hipStream_t st);
+int64_t embed_grad_ws_bytes(int64_t n, int64_t vocab, int64_t dim);
+int launch_embed(const kd_embed_args& a, hipStream_t st);
+int launch_embed_grad(const kd_embed_args& a, uint8_t* ws, hipStream_t st);
 int launch_signs(const uint64_t* bits, int d, float* out, hipStream_t st);
 int launch_span_count(const kd_span_args& a, int32_t* counts, hipStream_t st);
 int launch_span(const kd_span_args& a, hipStream_t st);

@@ -13,7 +13,7 @@
 // piece-major, so an XCD's workgroups read the same tokens through its L2.
 #include <cmath>
 
-#include "kd_tile.h"
+#include "kd_block8.h"
 
 namespace kd {
 namespace {
@@ -135,6 +135,129 @@ __global__ __launch_bounds__(256) void k_wgrad_sum(const float* __restrict__ par
   *reinterpret_cast<u32x4*>(dw + i) = pack8<E>(f);
 }
 
+// The same with X in 8-bit blocks (kd_block8.h), the checkpoint that a forward
+// kept: dW [N, K] = dY^T X.  Tiles of dW are 128 columns of K wide, a block's
+// width, so a row of an X tile has one scale: a thread takes 32 bytes of a row,
+// multiplies them out to bf16 -- exactly, 4 bits and a power of two -- and writes
+// them where the 16-bit kernel's copy would have put them.  A dY in fp16 enters
+// as two bf16 (8 + 8 of its 11 bits), since X's range does not fit fp16.
+struct Wgrad8Args {
+  WgradArgs w;
+  const uint8_t* scale;
+  int64_t ldx;
+  int ldy, nb;
+};
+
+template <class E>
+__global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args g) {
+  using TL = Tile<WT, 4>;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_y[2][TL::BYTES];
+  __shared__ __attribute__((aligned(1024))) uint8_t s_x[2][TL::BYTES];
+  const WgradArgs& w = g.w;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hf = lane >> 5,
+            c = lane & 31;
+  const int item = xcd_remap(blockIdx.x, gridDim.x), tiles = w.tn * w.tk;
+  const int piece = item / tiles, tile = item - piece * tiles;
+  const int n0 = (tile / w.tk) * WT, kb = tile - (tile / w.tk) * w.tk, k0 = kb * WT;
+  const int steps_all = (w.M + 63) / 64;
+  const int e0 = int(int64_t(steps_all) * piece / w.S), e1 = int(int64_t(steps_all) * (piece + 1) / w.S);
+  const uint32_t yrb = uint32_t(g.ldy) * 2u;
+  uint32_t yoff[TL::LOADS_PER_WAVE];
+  TL::load_offsets(wave, lane, yrb, yoff, uint32_t(w.N - n0) * 2u);
+  const int xr = tid >> 2, xc = k0 + (tid & 3) * 32;  // this thread's row of a step and its first column
+  u32x4 xv[2];
+  uint32_t xs = 0;
+  auto load = [&](int e, int slot) {
+    const int rows = min(64, w.M - e * 64);
+    const u32x4 rs = rsrc_words(static_cast<const uint16_t*>(w.dy) + int64_t(e) * 64 * g.ldy,
+                                uint32_t(int64_t(rows - 1) * yrb + uint32_t(w.N) * 2u));
+    TL::load_async(rs, uint32_t(n0) * 2u, yoff, lds_addr(s_y[slot]), wave);
+    xv[0] = xv[1] = u32x4{}, xs = 0;
+    if (xr < rows) {
+      const int64_t row = int64_t(e) * 64 + xr;
+      const uint8_t* p = static_cast<const uint8_t*>(w.x) + row * g.ldx + xc;
+      if (xc < w.K) xv[0] = *reinterpret_cast<const u32x4*>(p), xs = g.scale[row * g.nb + kb];
+      if (xc + 16 < w.K) xv[1] = *reinterpret_cast<const u32x4*>(p + 16);
+    }
+  };
+  auto put = [&](int slot) {
+    const float s = scale_value(xs);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float f[8];
+      unpack_e4m3(u32x2{xv[q >> 1][2 * (q & 1)], xv[q >> 1][2 * (q & 1) + 1]}, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] *= s;
+      *reinterpret_cast<u32x4*>(s_x[slot] + TL::at(xr, 4 * (tid & 3) + q)) = pack8<BF16>(f);
+    }
+  };
+  const int wn = wave >> 1, wk = wave & 1;
+  int ya[2][2], xa[2][2];
+  {
+    const int i = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = 8 * (q >> 1) + 4 * half + (i >> 2), ch = 2 * (q & 1) + ((i & 3) >> 1);
+        ya[b][half] = TL::at(r, 4 * (2 * wn + b) + ch) + 8 * (i & 1);
+        xa[b][half] = TL::at(r, 4 * (2 * wk + b) + ch) + 8 * (i & 1);
+      }
+  }
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) acc[a][b] = f32x16{};
+  if (e0 < e1) load(e0, 0);
+  for (int e = e0; e < e1; ++e) {
+    const int slot = (e - e0) & 1;
+    wait_vmem();
+    settle(xv[0]), settle(xv[1]), settle(xs);
+    put(slot);
+    barrier_lds();  // the step's tiles are in place for every wave, and every wave is done with the other slot
+    if (e + 1 < e1) load(e + 1, slot ^ 1);
+    lds_u8 *ty = to_lds(s_y[slot]), *tx = to_lds(s_x[slot]);
+    auto read = [&](lds_u8* t, const int (&at)[2], int ks) {
+      const u32x2 lo = ds_read_tr16(t + at[0] + ks * 16 * TL::ROWB);
+      const u32x2 hi = ds_read_tr16(t + at[1] + ks * 16 * TL::ROWB);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      u32x4 av[2], bv[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) av[b] = read(ty, ya[b], ks), bv[b] = read(tx, xa[b], ks);
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        u32x4 hi = av[a];
+        if constexpr (std::is_same_v<E, F16>) {
+          float f[8];
+          unpack8<F16>(av[a], f);
+          hi = pack8<BF16>(f);
+          const u32x4 lo = pack8_residual<BF16>(f, hi);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) acc[a][b] = mfma32x32x16<BF16>(lo, bv[b], acc[a][b]);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) acc[a][b] = mfma32x32x16<BF16>(hi, bv[b], acc[a][b]);
+      }
+    }
+  }
+  float* out = w.part + int64_t(piece) * w.N * w.K;
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int k = k0 + 64 * wk + 32 * b + c;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int n = n0 + 64 * wn + 32 * a + 8 * (r >> 2) + 4 * hf + (r & 3);
+        if (n < w.N && k < w.K) out[int64_t(n) * w.K + k] = acc[a][b][r];
+      }
+    }
+}
+
 }  // namespace
 
 // Pieces: a step of 64 tokens takes a workgroup 0.45 us with two on a CU, and a
@@ -156,6 +279,24 @@ int launch_wgrad(const void* dy, const void* x, void* dw, float* part, int M, in
                        static_cast<uint16_t*>(dw), n, w.S);
   };
   if (dtype == KD_BF16) go(BF16{});
+  else go(F16{});
+  return hipGetLastError() == hipSuccess ? KD_OK : KD_ERR_LAUNCH;
+}
+
+int64_t wgrad8_ws_bytes(int M, int N, int K) { return int64_t(4) * wgrad_pieces(M, N, K) * N * K; }
+
+int launch_wgrad8(const kd_wgrad8_args& a, hipStream_t st) {
+  const int S = wgrad_pieces(a.M, a.N, a.K);
+  Wgrad8Args g{{a.dy, a.x, a.ws, a.M, a.N, a.K, S, (a.N + WT - 1) / WT, (a.K + WT - 1) / WT}, a.x_scale, a.ldx, int(a.ldy),
+               (a.K + QB - 1) / QB};
+  const int64_t n = int64_t(a.N) * a.K;
+  auto go = [&](auto e) {
+    using E = decltype(e);
+    hipLaunchKernelGGL(k_wgrad8<E>, dim3(unsigned(g.w.tn * g.w.tk * S)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL(k_wgrad_sum<E>, dim3(unsigned((n / 8 + 255) / 256)), dim3(256), 0, st, a.ws,
+                       static_cast<uint16_t*>(a.dw), n, S);
+  };
+  if (a.dtype == KD_BF16) go(BF16{});
   else go(F16{});
   return hipGetLastError() == hipSuccess ? KD_OK : KD_ERR_LAUNCH;
 }
