@@ -295,15 +295,17 @@ typedef struct {
 } kd_gate8_args;
 
 typedef struct {
-  const void *dy;           /* [M, N] bf16 / fp16, rows ldy elements apart (a multiple of 8) */
-  int64_t ldy;
+  const void *dy[4];        /* n parts side by side: [M, cols[i]] bf16 / fp16, all but the last a multiple of 128 wide */
+  int64_t ldy[4];           /* rows apart, in elements, a multiple of 8 */
+  int32_t cols[4];          /* multiples of 8 */
+  int32_t n, pad_;          /* 1 .. 4 */
   const uint8_t *x;         /* [M, K] e4m3, rows ldx bytes apart */
   int64_t ldx;
   const uint8_t *x_scale;   /* [M, ceil(K / 128)] */
   void *dw;                 /* [N, K] contiguous, dy's type */
   float *ws;                /* kd_weight_grad8_ws_bytes, used by this call alone */
   int64_t ws_bytes;
-  int32_t M, N, K, dtype;   /* N and K multiples of 8 */
+  int32_t M, N, K, dtype;   /* N: sum of cols; K a multiple of 8 */
 } kd_wgrad8_args;
 
 typedef struct {

@@ -182,8 +182,8 @@ class Wgrad8Args(ctypes.Structure):
     """Mirror of ``kd_wgrad8_args``."""
 
     _fields_ = [
-        ("dy", c_void_p), ("ldy", c_int64), ("x", c_void_p), ("ldx", c_int64), ("x_scale", c_void_p), ("dw", c_void_p),
-        ("ws", c_void_p), ("ws_bytes", c_int64), ("M", c_int32), ("N", c_int32), ("K", c_int32), ("dtype", c_int32),
+        ("dy", c_void_p * 4), ("ldy", c_int64 * 4), ("cols", c_int32 * 4), ("n", c_int32), ("pad_", c_int32),
+        ("x", c_void_p), ("ldx", c_int64), ("x_scale", c_void_p), ("dw", c_void_p), ("ws", c_void_p), ("ws_bytes", c_int64), ("M", c_int32), ("N", c_int32), ("K", c_int32), ("dtype", c_int32),
     ]
 
 

@@ -50,7 +50,7 @@ _SCHEMAS = {
     "norm8_bwd": "(Tensor g, Tensor? ds, Tensor y, Tensor scale, Tensor rstd) -> Tensor",
     "gate8": "(Tensor a, Tensor b, bool keep) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
     "gate8_bwd": "(Tensor dy, Tensor a, Tensor a_scale, Tensor b, Tensor b_scale) -> (Tensor, Tensor)",
-    "weight_grad8": "(Tensor dy, Tensor x, Tensor x_scale, int K) -> Tensor",
+    "weight_grad8": "(Tensor[] dy, Tensor x, Tensor x_scale, int K) -> Tensor",
 }
 for _name, _schema in _SCHEMAS.items():
     torch.library.define(f"kdattn::{_name}", _schema)
@@ -126,8 +126,8 @@ def _(dy, a, a_scale, b, b_scale):
 
 
 @_fake("weight_grad8")
-def _(dy, x, x_scale, K):
-    return dy.new_empty((dy.shape[1], K))
+def _(dys, x, x_scale, K):
+    return dys[0].new_empty((sum(d.shape[1] for d in dys), K))
 
 
 def _ops():
@@ -283,11 +283,16 @@ def _cotangents(dys, sizes, like):
 def _backward_products(ctx, dys, x8, xs, wt, wts, want_x, want_w):
     """(gradient of the 8-bit operand, gradients of the weights)."""
     ops = torch.ops.kdattn
-    dx = None
+    dx, dws, at = None, [], 0
+    parts = _stacked(dys, 1)
     if want_x:
-        d8, ds = ops.quant_rows8(_stacked(dys, 1))
+        d8, ds = ops.quant_rows8(parts)
         dx = ops.matmul8(d8, ds, wt, wts, ctx.dtype)
-    return dx, [ops.weight_grad8(d, x8, xs, ctx.k) if w else None for d, w in zip(dys, want_w)]
+    dw = ops.weight_grad8(parts, x8, xs, ctx.k) if any(want_w) else None
+    for d, want in zip(dys, want_w):
+        dws.append(dw[at:at + d.shape[1]] if want else None)
+        at += d.shape[1]
+    return dx, dws
 
 
 class _NormProjection(torch.autograd.Function):

@@ -387,8 +387,16 @@ int kd_weight_grad8(const kd_wgrad8_args* a, void* stream) {
   int r;
   if (a == nullptr) return fail(KD_ERR_INVALID, "args is NULL");
   if ((r = check_wgrad8(a->M, a->N, a->K, a->dtype)) || (r = check_flat({a->dw, a->ws}))) return r;
-  if ((r = check_source(a->dy, a->ldy, a->N)) || (r = check_rows8(a->x, a->ldx, a->K))) return r;
-  if (a->ldy > (1 << 23)) return fail(KD_ERR_UNSUPPORTED, "dy's rows must be <= 2^23 elements apart");
+  if (a->n < 1 || a->n > 4) return fail(KD_ERR_INVALID, "n must be in 1 .. 4");
+  int64_t total = 0;
+  for (int i = 0; i < a->n; ++i) {
+    if ((r = check_count(a->M, a->cols[i])) || (r = check_source(a->dy[i], a->ldy[i], a->cols[i]))) return r;
+    if (a->ldy[i] > (1 << 23)) return fail(KD_ERR_UNSUPPORTED, "dy's rows must be <= 2^23 elements apart");
+    if (i + 1 < a->n && a->cols[i] % 128 != 0) return fail(KD_ERR_INVALID, "parts before the last must be whole tiles of 128");
+    total += a->cols[i];
+  }
+  if (total != a->N) return fail(KD_ERR_INVALID, "N must be the sum of cols");
+  if ((r = check_rows8(a->x, a->ldx, a->K))) return r;
   if (a->x_scale == nullptr) return fail(KD_ERR_INVALID, "x_scale is required");
   if (a->ws_bytes < kd::wgrad8_ws_bytes(a->M, a->N, a->K)) return fail(KD_ERR_INVALID, "ws is too small");
   r = kd::launch_wgrad8(*a, as_stream(stream));

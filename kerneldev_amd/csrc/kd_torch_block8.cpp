@@ -228,26 +228,37 @@ std::tuple<Tensor, Tensor> gate8_bwd(const Tensor& dy_in, const Tensor& a8, cons
   return {da, db};
 }
 
-// dy^T times the `K` columns that x8 holds
-Tensor weight_grad8(const Tensor& dy_in, const Tensor& x, const Tensor& x_scale, int64_t K) {
-  on_one_gpu({&dy_in, &x, &x_scale});
-  const c10::DeviceGuard on(dy_in.device());
-  const Tensor dy = rows_ready(dy_in);
-  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == dy.size(0), "dy [M, N] and x [M, K] expected, got ", dy.sizes(), " and ", x.sizes());
-  check_blocks(x, x_scale, K, 1, "x");
-  const int64_t M = dy.size(0), N = dy.size(1);
-  TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31), "M and N must be < 2^31");
+// The parts of dy, stacked, transposed, times the `K` columns that x8 holds
+Tensor weight_grad8(at::TensorList dys, const Tensor& x, const Tensor& x_scale, int64_t K) {
+  TORCH_CHECK_VALUE(!dys.empty() && dys.size() <= 4, "1 to 4 parts are expected");
+  on_one_gpu({&dys[0], &x, &x_scale});
+  const c10::DeviceGuard on(x.device());
   kd_wgrad8_args g{};
-  g.dtype = dtype_code(dy.scalar_type(), false);
-  if (M == 0) return at::zeros({N, K}, dy.options());
-  Tensor dw = at::empty({N, K}, dy.options());
+  std::vector<Tensor> keep;
+  int64_t N = 0;
+  for (const Tensor& d : dys) {
+    on_one_gpu({&x, &d});
+    keep.push_back(rows_ready(d));
+    const Tensor& dy = keep.back();
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == dy.size(0) && dy.scalar_type() == dys[0].scalar_type(),
+                      "dy [M, N] of one type and x [M, K] expected, got ", dy.sizes(), " and ", x.sizes());
+    TORCH_CHECK_VALUE(dy.size(1) < (int64_t(1) << 31), "N must be < 2^31");
+    g.dy[g.n] = dy.data_ptr(), g.ldy[g.n] = dy.stride(0), g.cols[g.n] = int32_t(dy.size(1)), ++g.n;
+    N += dy.size(1);
+  }
+  check_blocks(x, x_scale, K, 1, "x");
+  const int64_t M = x.size(0);
+  TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31), "M and N must be < 2^31");
+  g.dtype = dtype_code(dys[0].scalar_type(), false);
+  if (M == 0) return at::zeros({N, K}, dys[0].options());
+  Tensor dw = at::empty({N, K}, dys[0].options());
   g.M = int32_t(M), g.N = int32_t(N), g.K = int32_t(K);
   g.ws_bytes = kd_weight_grad8_ws_bytes(g.M, g.N, g.K, g.dtype);
   check(g.ws_bytes < 0 ? KD_ERR_UNSUPPORTED : KD_OK, "kd_weight_grad8");
-  const Tensor ws = at::empty({g.ws_bytes}, dy.options().dtype(at::kByte));
-  g.dy = dy.data_ptr(), g.ldy = dy.stride(0), g.x = u8(x), g.ldx = x.stride(0), g.x_scale = u8(x_scale);
+  const Tensor ws = at::empty({g.ws_bytes}, dys[0].options().dtype(at::kByte));
+  g.x = u8(x), g.ldx = x.stride(0), g.x_scale = u8(x_scale);
   g.dw = dw.data_ptr(), g.ws = static_cast<float*>(ws.data_ptr());
-  check(kd_weight_grad8(&g, stream_of(dy)), "kd_weight_grad8");
+  check(kd_weight_grad8(&g, stream_of(x)), "kd_weight_grad8");
   return dw;
 }
 

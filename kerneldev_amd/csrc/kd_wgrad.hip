@@ -136,24 +136,35 @@ __global__ __launch_bounds__(256) void k_wgrad_sum(const float* __restrict__ par
 }
 
 // The same with X in 8-bit blocks (kd_block8.h), the checkpoint that a forward
-// kept: dW [N, K] = dY^T X.  Tiles of dW are 128 columns of K wide, a block's
-// width, so a row of an X tile has one scale: a thread takes 32 bytes of a row,
-// multiplies them out to bf16 -- exactly, 4 bits and a power of two -- and writes
-// them where the 16-bit kernel's copy would have put them.  A dY in fp16 enters
+// kept: dW [N, K] = dY^T X, dY in up to four parts side by side.  Tiles of dW are
+// 128 columns of K wide, a block's width, so a row of an X tile has one scale: a
+// thread takes 32 bytes of a row, multiplies them out to bf16 -- exactly, 4 bits and
+// a power of two -- and writes them where the 16-bit kernel's copy would have put
+// them, a step ahead, between the products of the step before.  A dY in fp16 enters
 // as two bf16 (8 + 8 of its 11 bits), since X's range does not fit fp16.
 struct Wgrad8Args {
-  WgradArgs w;
-  const uint8_t* scale;
+  const void* dy[4];
+  int64_t ldy[4];
+  int cols[4], n;
+  const uint8_t *x, *scale;
   int64_t ldx;
-  int ldy, nb;
+  float* part;
+  int M, N, K, S, tn, tk, nb;
 };
 
+// 16 e4m3 bytes times the scale as 16 bf16
+KD_DEV void widen16(const u32x4& v, float scale, u32x4 (&out)[2]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    out[i >> 2][i & 3] = __builtin_bit_cast(uint32_t, (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i >> 1], scale, true)
+                                                              : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i >> 1], scale, false));
+}
+
 template <class E>
-__global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args g) {
+__global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args w) {
   using TL = Tile<WT, 4>;
   __shared__ __attribute__((aligned(1024))) uint8_t s_y[2][TL::BYTES];
   __shared__ __attribute__((aligned(1024))) uint8_t s_x[2][TL::BYTES];
-  const WgradArgs& w = g.w;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hf = lane >> 5,
             c = lane & 31;
   const int item = xcd_remap(blockIdx.x, gridDim.x), tiles = w.tn * w.tk;
@@ -161,34 +172,41 @@ __global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args g) {
   const int n0 = (tile / w.tk) * WT, kb = tile - (tile / w.tk) * w.tk, k0 = kb * WT;
   const int steps_all = (w.M + 63) / 64;
   const int e0 = int(int64_t(steps_all) * piece / w.S), e1 = int(int64_t(steps_all) * (piece + 1) / w.S);
-  const uint32_t yrb = uint32_t(g.ldy) * 2u;
+  // dY's part that holds the tile (parts before the last are whole tiles)
+  const uint8_t* dy = static_cast<const uint8_t*>(w.dy[0]);
+  int64_t ldy = w.ldy[0];
+  int cols = w.cols[0], first = n0;
+#pragma unroll
+  for (int i = 1; i < 4; ++i)
+    if (i < w.n && first >= cols) first -= cols, dy = static_cast<const uint8_t*>(w.dy[i]), ldy = w.ldy[i], cols = w.cols[i];
+  const uint32_t yrb = uint32_t(ldy) * 2u;
   uint32_t yoff[TL::LOADS_PER_WAVE];
-  TL::load_offsets(wave, lane, yrb, yoff, uint32_t(w.N - n0) * 2u);
-  const int xr = tid >> 2, xc = k0 + (tid & 3) * 32;  // this thread's row of a step and its first column
-  u32x4 xv[2];
-  uint32_t xs = 0;
-  auto load = [&](int e, int slot) {
-    const int rows = min(64, w.M - e * 64);
-    const u32x4 rs = rsrc_words(static_cast<const uint16_t*>(w.dy) + int64_t(e) * 64 * g.ldy,
-                                uint32_t(int64_t(rows - 1) * yrb + uint32_t(w.N) * 2u));
-    TL::load_async(rs, uint32_t(n0) * 2u, yoff, lds_addr(s_y[slot]), wave);
-    xv[0] = xv[1] = u32x4{}, xs = 0;
-    if (xr < rows) {
-      const int64_t row = int64_t(e) * 64 + xr;
-      const uint8_t* p = static_cast<const uint8_t*>(w.x) + row * g.ldx + xc;
-      if (xc < w.K) xv[0] = *reinterpret_cast<const u32x4*>(p), xs = g.scale[row * g.nb + kb];
-      if (xc + 16 < w.K) xv[1] = *reinterpret_cast<const u32x4*>(p + 16);
-    }
+  TL::load_offsets(wave, lane, yrb, yoff, uint32_t(cols - first) * 2u);
+  auto load_y = [&](int e, int slot) {
+    const int rows = max(0, min(64, w.M - e * 64));
+    const u32x4 rs = rsrc_words(dy + int64_t(e) * 64 * yrb, rows > 0 ? uint32_t(rows - 1) * yrb + uint32_t(cols) * 2u : 0u);
+    TL::load_async(rs, uint32_t(first) * 2u, yoff, lds_addr(s_y[slot]), wave);
   };
-  auto put = [&](int slot) {
+  const int xr = tid >> 2, xc = k0 + (tid & 3) * 32;  // this thread's row of a step and its first column
+  const uint32_t xo[2] = {xc < w.K ? uint32_t(xr * w.ldx) + xc : OFF_OUTSIDE, xc + 16 < w.K ? uint32_t(xr * w.ldx) + xc + 16 : OFF_OUTSIDE};
+  u32x4 xv[2];
+  uint32_t xs;
+  auto load_x = [&](int e) {  // (rows and columns outside: zeros)
+    const int rows = max(0, min(64, w.M - e * 64));
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(w.x + int64_t(e) * 64 * w.ldx, rows > 0 ? uint32_t((rows - 1) * w.ldx + (w.K + 15) / 16 * 16) : 0u),
+                                 rsc = make_rsrc(w.scale + int64_t(e) * 64 * w.nb, uint32_t(rows * w.nb));
+#pragma unroll
+    for (int q = 0; q < 2; ++q) xv[q] = buf_load16(r, xo[q]);
+    xs = __builtin_amdgcn_raw_buffer_load_b8(rsc, uint32_t(xr * w.nb + kb), 0, 0);
+  };
+  auto put_x = [&](int slot) {
     const float s = scale_value(xs);
+    u32x4 o[2];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float f[8];
-      unpack_e4m3(u32x2{xv[q >> 1][2 * (q & 1)], xv[q >> 1][2 * (q & 1) + 1]}, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= s;
-      *reinterpret_cast<u32x4*>(s_x[slot] + TL::at(xr, 4 * (tid & 3) + q)) = pack8<BF16>(f);
+    for (int q = 0; q < 2; ++q) {
+      widen16(xv[q], s, o);
+      *reinterpret_cast<u32x4*>(s_x[slot] + TL::at(xr, 4 * (tid & 3) + 2 * q)) = o[0];
+      *reinterpret_cast<u32x4*>(s_x[slot] + TL::at(xr, 4 * (tid & 3) + 2 * q + 1)) = o[1];
     }
   };
   const int wn = wave >> 1, wk = wave & 1;
@@ -209,41 +227,56 @@ __global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args g) {
   for (int a = 0; a < 2; ++a)
 #pragma unroll
     for (int b = 0; b < 2; ++b) acc[a][b] = f32x16{};
-  if (e0 < e1) load(e0, 0);
-  for (int e = e0; e < e1; ++e) {
+  load_x(e0);
+  load_y(e0, 0);
+  wait_vmem();
+  settle(xv[0]), settle(xv[1]), settle(xs);
+  put_x(0);
+  load_x(e0 + 1);
+  for (int e = e0; e < e1; ++e) {  // (one basic block: copies of a step behind the piece are read by nobody)
     const int slot = (e - e0) & 1;
     wait_vmem();
     settle(xv[0]), settle(xv[1]), settle(xs);
-    put(slot);
     barrier_lds();  // the step's tiles are in place for every wave, and every wave is done with the other slot
-    if (e + 1 < e1) load(e + 1, slot ^ 1);
+    load_y(e + 1, slot ^ 1);
     lds_u8 *ty = to_lds(s_y[slot]), *tx = to_lds(s_x[slot]);
     auto read = [&](lds_u8* t, const int (&at)[2], int ks) {
       const u32x2 lo = ds_read_tr16(t + at[0] + ks * 16 * TL::ROWB);
       const u32x2 hi = ds_read_tr16(t + at[1] + ks * 16 * TL::ROWB);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
+    u32x4 av[2][2], bv[2][2];  // [k-step parity][block]
+#pragma unroll
+    for (int b = 0; b < 2; ++b) av[0][b] = read(ty, ya[b], 0), bv[0][b] = read(tx, xa[b], 0);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-      u32x4 av[2], bv[2];
+      __builtin_amdgcn_sched_barrier(0x406);
+      if (ks + 1 < 4) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) av[b] = read(ty, ya[b], ks), bv[b] = read(tx, xa[b], ks);
+        for (int b = 0; b < 2; ++b)
+          av[(ks + 1) & 1][b] = read(ty, ya[b], ks + 1), bv[(ks + 1) & 1][b] = read(tx, xa[b], ks + 1);
+      }
+      if (ks == 1) put_x(slot ^ 1);
+      if (ks == 2) load_x(e + 2);
+      __builtin_amdgcn_sched_barrier(0x406);
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        u32x4 hi = av[a];
+        u32x4 hi = av[ks & 1][a];
         if constexpr (std::is_same_v<E, F16>) {
           float f[8];
-          unpack8<F16>(av[a], f);
+          unpack8<F16>(hi, f);
           hi = pack8<BF16>(f);
           const u32x4 lo = pack8_residual<BF16>(f, hi);
 #pragma unroll
-          for (int b = 0; b < 2; ++b) acc[a][b] = mfma32x32x16<BF16>(lo, bv[b], acc[a][b]);
+          for (int b = 0; b < 2; ++b) acc[a][b] = mfma32x32x16<BF16>(lo, bv[ks & 1][b], acc[a][b]);
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) acc[a][b] = mfma32x32x16<BF16>(hi, bv[b], acc[a][b]);
+        for (int b = 0; b < 2; ++b) acc[a][b] = mfma32x32x16<BF16>(hi, bv[ks & 1][b], acc[a][b]);
       }
     }
+    __builtin_amdgcn_sched_barrier(0x406);
   }
+  wait_vmem();  // (the copies behind the piece land before the LDS is given back)
   float* out = w.part + int64_t(piece) * w.N * w.K;
 #pragma unroll
   for (int a = 0; a < 2; ++a)
@@ -287,12 +320,15 @@ int64_t wgrad8_ws_bytes(int M, int N, int K) { return int64_t(4) * wgrad_pieces(
 
 int launch_wgrad8(const kd_wgrad8_args& a, hipStream_t st) {
   const int S = wgrad_pieces(a.M, a.N, a.K);
-  Wgrad8Args g{{a.dy, a.x, a.ws, a.M, a.N, a.K, S, (a.N + WT - 1) / WT, (a.K + WT - 1) / WT}, a.x_scale, a.ldx, int(a.ldy),
-               (a.K + QB - 1) / QB};
+  Wgrad8Args g{};
+  for (int i = 0; i < a.n; ++i) g.dy[i] = a.dy[i], g.ldy[i] = a.ldy[i], g.cols[i] = a.cols[i];
+  g.n = a.n, g.x = a.x, g.scale = a.x_scale, g.ldx = a.ldx, g.part = a.ws;
+  g.M = a.M, g.N = a.N, g.K = a.K, g.S = S;
+  g.tn = (a.N + WT - 1) / WT, g.tk = (a.K + WT - 1) / WT, g.nb = (a.K + QB - 1) / QB;
   const int64_t n = int64_t(a.N) * a.K;
   auto go = [&](auto e) {
     using E = decltype(e);
-    hipLaunchKernelGGL(k_wgrad8<E>, dim3(unsigned(g.w.tn * g.w.tk * S)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL(k_wgrad8<E>, dim3(unsigned(g.tn * g.tk * S)), dim3(256), 0, st, g);
     hipLaunchKernelGGL(k_wgrad_sum<E>, dim3(unsigned((n / 8 + 255) / 256)), dim3(256), 0, st, a.ws,
                        static_cast<uint16_t*>(a.dw), n, S);
   };

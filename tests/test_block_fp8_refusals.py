@@ -88,7 +88,7 @@ GOOD = {
     "kd_gate8": (_lib.Gate8Args, dict(a=P, b=P, a_stride=64, b_stride=64, y8=P, y_scale=P, a8=P, a_scale=P, b8=P, b_scale=P,
                                       stride=64, rows=4, H=64, dtype=0)),
     "kd_gate8_bwd": (_lib.Gate8Args, dict(dy=P, da=P, db=P, a8=P, a_scale=P, b8=P, b_scale=P, stride=64, rows=4, H=64, dtype=0)),
-    "kd_weight_grad8": (_lib.Wgrad8Args, dict(dy=P, ldy=16, x=P, ldx=64, x_scale=P, dw=P, ws=P, ws_bytes=1 << 40, M=4, N=16,
+    "kd_weight_grad8": (_lib.Wgrad8Args, dict(dy=[P], ldy=[16], cols=[16], n=1, x=P, ldx=64, x_scale=P, dw=P, ws=P, ws_bytes=1 << 40, M=4, N=16,
                                               K=64, dtype=0)),
     "kd_embed": (_lib.EmbedArgs, dict(tokens=P, n=5, weight=P, out=P, vocab=7, dim=16, padding_idx=-1, tokens_dtype=0, dtype=0)),
     "kd_embed_grad": (_lib.EmbedArgs, dict(tokens=P, n=5, dy=P, dw=P, vocab=7, dim=16, padding_idx=-1, tokens_dtype=0, dtype=0)),
@@ -117,8 +117,9 @@ INVALID, UNSUPPORTED = _lib.KD_ERR_INVALID, _lib.KD_ERR_UNSUPPORTED
     ("kd_norm8_bwd", dict(rstd=None), INVALID), ("kd_norm8_bwd", dict(dx=None), INVALID), ("kd_norm8_bwd", dict(ds=P + 4), INVALID),
     ("kd_gate8", dict(H=60), UNSUPPORTED), ("kd_gate8", dict(a_stride=56), INVALID), ("kd_gate8", dict(b8=None), INVALID),
     ("kd_gate8", dict(y_scale=None), INVALID), ("kd_gate8_bwd", dict(a8=None), INVALID), ("kd_gate8_bwd", dict(da=P + 2), INVALID),
-    ("kd_weight_grad8", dict(N=12), UNSUPPORTED), ("kd_weight_grad8", dict(M=0), INVALID), ("kd_weight_grad8", dict(ws_bytes=16), INVALID),
-    ("kd_weight_grad8", dict(ldy=12), INVALID), ("kd_weight_grad8", dict(dtype=2), UNSUPPORTED), ("kd_weight_grad8", dict(x_scale=None), INVALID),
+    ("kd_weight_grad8", dict(N=12), UNSUPPORTED), ("kd_weight_grad8", dict(N=24), INVALID), ("kd_weight_grad8", dict(n=0), INVALID),
+    ("kd_weight_grad8", dict(n=2, dy=[P, P], ldy=[16, 16], cols=[16, 16], N=32), INVALID), ("kd_weight_grad8", dict(M=0), INVALID), ("kd_weight_grad8", dict(ws_bytes=16), INVALID),
+    ("kd_weight_grad8", dict(ldy=[12]), INVALID), ("kd_weight_grad8", dict(dy=[P + 8]), INVALID), ("kd_weight_grad8", dict(dtype=2), UNSUPPORTED), ("kd_weight_grad8", dict(x_scale=None), INVALID),
     ("kd_embed", dict(n=0), UNSUPPORTED), ("kd_embed", dict(vocab=0), UNSUPPORTED), ("kd_embed", dict(dim=0), UNSUPPORTED),
     ("kd_embed", dict(tokens=None), INVALID), ("kd_embed", dict(tokens_dtype=2), INVALID), ("kd_embed", dict(dtype=3), UNSUPPORTED),
     ("kd_embed", dict(weight=None), INVALID), ("kd_embed_grad", dict(dy=None), INVALID), ("kd_embed_grad", dict(dw=P + 2), INVALID),

@@ -389,6 +389,31 @@ def test_parts_of_the_gradient(dev):
     assert z.shape == (0, 9, 128) and not gz.any() and not gw.any()
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 24, 24), (44, 72, 264), (65, 128, 128), (300, 264, 768), (1000, 1000, 528)])
+def test_memory_around_the_operands(dev, m, n, k):
+    """NaN before and behind the rows and columns of every operand: no value of it comes in."""
+    def within(t):
+        big = torch.full((t.shape[0] + 80, t.shape[1] + 64), 0x7F if t.element_size() == 1 else 0x7FC0,
+                         dtype=torch.uint8 if t.element_size() == 1 else torch.int16, device=dev).view(t.dtype)
+        v = big[40:40 + t.shape[0], 32:32 + t.shape[1]]
+        v.copy_(t)
+        return v
+
+    ops = torch.ops.kdattn
+    x, w, dy = (_data(s, torch.bfloat16, dev, 1) for s in ((m, k), (n, k), (m, n)))
+    x8, xs = ops.quant_rows8([x])
+    w8, ws, wt, wts = ops.quant_weight8([w], True)
+    d8, d_s = ops.quant_rows8([dy])
+    for a, b in zip(ops.quant_rows8([within(x)]) + ops.quant_weight8([within(w)], True), (x8, xs, w8, ws, wt, wts)):
+        assert torch.equal(a.float(), b.float())
+    for out in (torch.bfloat16, torch.float32):
+        assert torch.equal(ops.matmul8(within(x8), xs, within(w8), ws, out), ops.matmul8(x8, xs, w8, ws, out))
+        assert torch.equal(ops.matmul8(within(d8), d_s, within(wt), wts, out), ops.matmul8(d8, d_s, wt, wts, out))
+    assert torch.equal(ops.weight_grad8([within(dy)], within(x8), xs, k), ops.weight_grad8([dy], x8, xs, k))
+    for a, b in zip(ops.gate8(within(x), within(x), True), ops.gate8(x, x, True)):
+        assert torch.equal(a.float(), b.float())
+
+
 def test_same_bits_every_time(dev):
     x, w = _data((2000, 768), torch.bfloat16, dev, 1).requires_grad_(True), _data((768, 768), torch.bfloat16, dev, 2, 0.02).requires_grad_(True)
     dy = _data((2000, 768), torch.bfloat16, dev, 3, 0.01)
@@ -478,7 +503,7 @@ def test_compiled(dev):
                      (torch.ops.kdattn.quant_weight8, ([w1.detach(), w3.detach()], True)),
                      (torch.ops.kdattn.norm8, (x.detach(), d.detach(), 1e-6)),
                      (torch.ops.kdattn.gate8, (x.detach(), d.detach(), True)),
-                     (torch.ops.kdattn.weight_grad8, (dy, *torch.ops.kdattn.quant_rows8([x.detach()]), 256))):
+                     (torch.ops.kdattn.weight_grad8, ([dy], *torch.ops.kdattn.quant_rows8([x.detach()]), 256))):
         torch.library.opcheck(op, args, test_utils="test_faketensor")  # (test_schema multiplies: no float8 there)
 
 
@@ -499,6 +524,6 @@ def test_offsets_past_32_bits(dev):
     # the weight gradient reads all of it: a gradient that is zero but in those rows
     dy = torch.zeros(m, 8, device=dev, dtype=torch.bfloat16)
     dy[at] = torch.randn(at.numel(), 8, device=dev).bfloat16()
-    dw = torch.ops.kdattn.weight_grad8(dy, q.data, q.scale, k)
+    dw = torch.ops.kdattn.weight_grad8([dy], q.data, q.scale, k)
     kept = _values(kd.BlockFp8(q.data[at], q.scale[at]))
     _close(dw, dy[at].double().t() @ kept, at.numel() * 2.0 ** -23 * (dy[at].double().abs().t() @ kept.abs()))
