@@ -256,6 +256,7 @@ typedef struct {
   void *out;                /* [M, N], rows ldo elements apart */
   int64_t ldo;
   int32_t M, N, K, dtype;   /* K a multiple of 16; the type of out */
+  int32_t fast, pad_;       /* fp32 out: 1 takes the sums that 16-bit results are rounded from (about 1.4e-5 off) */
 } kd_matmul8_args;
 
 typedef struct {
@@ -272,14 +273,14 @@ typedef struct {
 } kd_norm8_args;
 
 typedef struct {
-  const void *g, *ds;       /* gradients of y and of sum (NULL: none), [rows, D] contiguous */
+  const void *g, *ds;       /* gradients of y (dtype, or fp32) and of sum (NULL: none), [rows, D] contiguous */
   const uint8_t *y;
   int64_t y_stride;
   const uint8_t *scale;
   const float *rstd;
   void *dx;                 /* the gradient of x, and of delta */
   int64_t rows;
-  int32_t D, dtype;
+  int32_t D, dtype, g_dtype, pad_;
 } kd_norm8_bwd_args;
 
 typedef struct {
@@ -288,10 +289,11 @@ typedef struct {
   uint8_t *y8, *y_scale;    /* forward: silu(a) b */
   uint8_t *a8, *a_scale, *b8, *b_scale; /* a and b: written (NULL: not kept), read by the backward */
   int64_t stride;           /* of all e4m3 rows */
-  const void *dy;           /* backward: [rows, H] contiguous, and the results alike */
+  const void *dy;           /* backward: [rows, H] contiguous (dtype, or fp32), and the results alike */
   void *da, *db;
   int64_t rows;
   int32_t H, dtype;         /* H a multiple of 8 */
+  int32_t dy_dtype, pad_;
 } kd_gate8_args;
 
 typedef struct {

@@ -145,6 +145,7 @@ class Matmul8Args(ctypes.Structure):
     _fields_ = [
         ("a", c_void_p), ("b", c_void_p), ("lda", c_int64), ("ldb", c_int64), ("a_scale", c_void_p), ("b_scale", c_void_p),
         ("out", c_void_p), ("ldo", c_int64), ("M", c_int32), ("N", c_int32), ("K", c_int32), ("dtype", c_int32),
+        ("fast", c_int32), ("pad_", c_int32),
     ]
 
 
@@ -164,6 +165,7 @@ class Norm8BwdArgs(ctypes.Structure):
     _fields_ = [
         ("g", c_void_p), ("ds", c_void_p), ("y", c_void_p), ("y_stride", c_int64), ("scale", c_void_p),
         ("rstd", c_void_p), ("dx", c_void_p), ("rows", c_int64), ("D", c_int32), ("dtype", c_int32),
+        ("g_dtype", c_int32), ("pad_", c_int32),
     ]
 
 
@@ -174,7 +176,7 @@ class Gate8Args(ctypes.Structure):
         ("a", c_void_p), ("b", c_void_p), ("a_stride", c_int64), ("b_stride", c_int64), ("y8", c_void_p),
         ("y_scale", c_void_p), ("a8", c_void_p), ("a_scale", c_void_p), ("b8", c_void_p), ("b_scale", c_void_p),
         ("stride", c_int64), ("dy", c_void_p), ("da", c_void_p), ("db", c_void_p), ("rows", c_int64), ("H", c_int32),
-        ("dtype", c_int32),
+        ("dtype", c_int32), ("dy_dtype", c_int32), ("pad_", c_int32),
     ]
 
 

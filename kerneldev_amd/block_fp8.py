@@ -45,11 +45,11 @@ class BlockFp8(NamedTuple):
 _SCHEMAS = {
     "quant_rows8": "(Tensor[] x) -> (Tensor, Tensor)",
     "quant_weight8": "(Tensor[] w, bool transpose) -> (Tensor, Tensor, Tensor, Tensor)",
-    "matmul8": "(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, ScalarType dtype) -> Tensor",
+    "matmul8": "(Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, ScalarType dtype, bool fast=False) -> Tensor",
     "norm8": "(Tensor x, Tensor? delta, float eps) -> (Tensor, Tensor, Tensor, Tensor)",
-    "norm8_bwd": "(Tensor g, Tensor? ds, Tensor y, Tensor scale, Tensor rstd) -> Tensor",
+    "norm8_bwd": "(Tensor g, Tensor? ds, Tensor y, Tensor scale, Tensor rstd, ScalarType dtype) -> Tensor",
     "gate8": "(Tensor a, Tensor b, bool keep) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)",
-    "gate8_bwd": "(Tensor dy, Tensor a, Tensor a_scale, Tensor b, Tensor b_scale) -> (Tensor, Tensor)",
+    "gate8_bwd": "(Tensor dy, Tensor a, Tensor a_scale, Tensor b, Tensor b_scale, ScalarType dtype) -> (Tensor, Tensor)",
     "weight_grad8": "(Tensor[] dy, Tensor x, Tensor x_scale, int K) -> Tensor",
 }
 for _name, _schema in _SCHEMAS.items():
@@ -95,7 +95,7 @@ def _(ws, transpose):
 
 
 @_fake("matmul8")
-def _(a, a_scale, b, b_scale, dtype):
+def _(a, a_scale, b, b_scale, dtype, fast=False):
     return a.new_empty((a.shape[0], b.shape[0]), dtype=dtype)
 
 
@@ -107,8 +107,8 @@ def _(x, delta, eps):
 
 
 @_fake("norm8_bwd")
-def _(g, ds, y, scale, rstd):
-    return torch.empty_like(g, memory_format=torch.contiguous_format)
+def _(g, ds, y, scale, rstd, dtype):
+    return g.new_empty(g.shape, dtype=dtype)
 
 
 @_fake("gate8")
@@ -120,9 +120,8 @@ def _(a, b, keep):
 
 
 @_fake("gate8_bwd")
-def _(dy, a, a_scale, b, b_scale):
-    return (torch.empty_like(dy, memory_format=torch.contiguous_format),
-            torch.empty_like(dy, memory_format=torch.contiguous_format))
+def _(dy, a, a_scale, b, b_scale, dtype):
+    return dy.new_empty(dy.shape, dtype=dtype), dy.new_empty(dy.shape, dtype=dtype)
 
 
 @_fake("weight_grad8")
@@ -157,6 +156,8 @@ def _check_gpu(name, *xs):
 def quantize_rows(x: torch.Tensor) -> BlockFp8:
     """``x`` ``[..., K]`` (bf16, fp16 or fp32; K a multiple of 16) in blocks of 128 columns of a row:
     data ``[..., K]`` and scale ``[..., ceil(K / 128)]``.  Not differentiable."""
+    if _lib.eager(x) and (got := _lib.native().quantize_rows(x)) is not None:
+        return BlockFp8(*got)
     _check_operand("x", x, (*_HALF, torch.float32), 16)
     _check_gpu("x", x)
     data, scale = _ops().quant_rows8([x.detach().reshape(-1, x.shape[-1])])
@@ -201,6 +202,8 @@ def fp8_matmul(a: BlockFp8, b: BlockFp8, out_dtype: torch.dtype = torch.bfloat16
     (:func:`quantize_weight`), fp32 sums, rounded once to ``out_dtype`` (bf16, fp16 or fp32).
 
     K is a multiple of 16; a single row of ``a`` is the form for one token.  Not differentiable."""
+    if _lib.eager(*a, *b) and (out := _lib.native().fp8_matmul(*a, *b, out_dtype)) is not None:
+        return out
     a, b = BlockFp8(*a), BlockFp8(*b)
     _check_blocks("a", a)
     _check_blocks("b", b, two_dim=True)
@@ -233,6 +236,8 @@ def add_rms_norm_fp8(x: torch.Tensor, delta: torch.Tensor | None = None, eps: fl
 
     ``x`` ``[..., D]`` bf16 or fp16, D a multiple of 16 up to 8192.  Not differentiable: training goes through
     :func:`norm_projection`."""
+    if _lib.eager(x, delta) and (got := _lib.native().add_rms_norm_fp8(x, delta, eps)) is not None:
+        return got[0], BlockFp8(*got[1:])
     _check_norm(x, delta, 16)
     _check_gpu("x", x)
     d = x.shape[-1]
@@ -280,14 +285,20 @@ def _cotangents(dys, sizes, like):
     return [like.new_zeros((like.shape[0], n)) if d is None else d.reshape(-1, n) for d, n in zip(dys, sizes)]
 
 
-def _backward_products(ctx, dys, x8, xs, wt, wts, want_x, want_w):
-    """(gradient of the 8-bit operand, gradients of the weights)."""
+def _between(dtype):
+    """The type of a gradient between two kernels: fp16, whose own rounding (2^-11) a second one would be felt beside, goes
+    through fp32; bf16 stays (half the bytes, an error of 1.4 times one rounding's)."""
+    return torch.float32 if dtype == torch.float16 else dtype
+
+
+def _backward_products(ctx, dys, x8, xs, wt, wts, want_x, want_w, dtype):
+    """(gradient of the 8-bit operand in ``dtype``, gradients of the weights)."""
     ops = torch.ops.kdattn
     dx, dws, at = None, [], 0
     parts = _stacked(dys, 1)
     if want_x:
         d8, ds = ops.quant_rows8(parts)
-        dx = ops.matmul8(d8, ds, wt, wts, ctx.dtype)
+        dx = ops.matmul8(d8, ds, wt, wts, dtype, True)
     dw = ops.weight_grad8(parts, x8, xs, ctx.k) if any(want_w) else None
     for d, want in zip(dys, want_w):
         dws.append(dw[at:at + d.shape[1]] if want else None)
@@ -317,10 +328,12 @@ class _NormProjection(torch.autograd.Function):
             return (dsum if want_x else None, dsum if want_d else None, None, *none)
         given = next(d for d in dys if d is not None)
         dys = _cotangents(dys, ctx.sizes, given.new_empty((y8.shape[0], 0)))
-        g, dws = _backward_products(ctx, dys, y8, ys, wt, wts, want_x or want_d, ctx.needs_input_grad[3:])
+        g, dws = _backward_products(ctx, dys, y8, ys, wt, wts, want_x or want_d, ctx.needs_input_grad[3:],
+                                    _between(ctx.dtype))
         dx = None
         if g is not None:
-            dx = torch.ops.kdattn.norm8_bwd(g, None if dsum is None else dsum.reshape(-1, ctx.k), y8, ys, rstd).view(ctx.shape)
+            dx = torch.ops.kdattn.norm8_bwd(g, None if dsum is None else dsum.reshape(-1, ctx.k), y8, ys, rstd,
+                                               ctx.dtype).view(ctx.shape)
         return (dx if want_x else None, dx if want_d else None, None, *dws)
 
 
@@ -331,6 +344,8 @@ def norm_projection(x: torch.Tensor, delta: torch.Tensor | None, *weights: torch
     ``x``, ``delta`` ``[..., K]`` and 1 to 4 ``weights`` ``[N_i, K]``, bf16 or fp16 of one type; K (up to 8192) and N_i
     multiples of 8.  The weights' blocks are those of all weights stacked.  Differentiable once; the backward
     keeps the normalised rows in 8 bits and one float a row.  The y_i are columns of one product, strided."""
+    if _lib.eager(x, delta, *weights) and (got := _lib.native().norm_projection(x, delta, weights, eps)) is not None:
+        return tuple(got)
     _check_norm(x, delta, 8)
     _check_weights(x, weights, x.shape[-1])
     _check_gpu("x", x)
@@ -354,13 +369,15 @@ class _Projection(torch.autograd.Function):
     def backward(ctx, dy):
         x8, xs, wt, wts = ctx.saved_tensors
         dx, (dw,) = _backward_products(ctx, [dy.reshape(-1, dy.shape[-1])], x8, xs, wt, wts, *ctx.needs_input_grad[:1],
-                                       ctx.needs_input_grad[1:])
+                                       ctx.needs_input_grad[1:], ctx.dtype)
         return None if dx is None else dx.view(ctx.shape), dw
 
 
 def fp8_projection(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
     """``x W^T`` of ``x`` ``[..., K]`` and ``weight`` ``[N, K]`` (bf16 or fp16; K, N multiples of 8) with both in
     8-bit blocks.  Differentiable once; the backward keeps ``x`` in 8 bits."""
+    if _lib.eager(x, weight) and (y := _lib.native().fp8_projection(x, weight)) is not None:
+        return y
     _check_operand("x", x)
     _check_weights(x, [weight], x.shape[-1])
     _check_gpu("x", x)
@@ -384,10 +401,11 @@ class _SwigluProjection(torch.autograd.Function):
     def backward(ctx, dy):
         y8, ys, a8, a_s, b8, b_s, wt, wts = ctx.saved_tensors
         want_a, want_b, want_w = ctx.needs_input_grad
-        g, (dw,) = _backward_products(ctx, [dy.reshape(-1, dy.shape[-1])], y8, ys, wt, wts, want_a or want_b, [want_w])
+        g, (dw,) = _backward_products(ctx, [dy.reshape(-1, dy.shape[-1])], y8, ys, wt, wts, want_a or want_b, [want_w],
+                                     _between(ctx.dtype))
         da = db = None
         if g is not None:
-            da, db = (t.view(ctx.shape) for t in torch.ops.kdattn.gate8_bwd(g, a8, a_s, b8, b_s))
+            da, db = (t.view(ctx.shape) for t in torch.ops.kdattn.gate8_bwd(g, a8, a_s, b8, b_s, ctx.dtype))
         return da if want_a else None, db if want_b else None, dw
 
 
@@ -395,6 +413,8 @@ def swiglu_projection(a: torch.Tensor, b: torch.Tensor, weight: torch.Tensor) ->
     """``(silu(a) b) W^T`` of ``a``, ``b`` ``[..., H]`` and ``weight`` ``[N, H]`` (bf16 or fp16; H, N multiples of 8),
     the gated rows and the weight in 8-bit blocks.  Differentiable once; the backward keeps ``a``, ``b`` and the
     gated rows in 8 bits each."""
+    if _lib.eager(a, b, weight) and (y := _lib.native().swiglu_projection(a, b, weight)) is not None:
+        return y
     _check_operand("a", a)
     if b.shape != a.shape or b.dtype != a.dtype or b.device != a.device:
         raise ValueError("a and b must have one shape, type and device")

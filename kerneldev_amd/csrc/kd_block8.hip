@@ -184,8 +184,8 @@ __global__ __launch_bounds__(256) void k_norm8(kd_norm8_args a, int64_t row0, in
   }
 }
 
-// dx = ds + r (g - y mean(g y)), y from its 8 bits
-template <class E, int NCH, int WPR>
+// dx = ds + r (g - y mean(g y)), y from its 8 bits; g in E or (EG) fp32
+template <class E, class EG, int NCH, int WPR>
 __global__ __launch_bounds__(256) void k_norm8_bwd(kd_norm8_bwd_args a, int64_t row0, int64_t end) {
   __shared__ float s_part[4];
   const int lane = threadIdx.x & (64 * WPR - 1);
@@ -193,12 +193,12 @@ __global__ __launch_bounds__(256) void k_norm8_bwd(kd_norm8_bwd_args a, int64_t 
   const int64_t row = at < end ? at : end - 1;
   const int words = a.D / 8;
   const int64_t nb = (a.D + QB - 1) / QB;
-  const u32x4* gp = static_cast<const u32x4*>(a.g) + row * words;
   float f[NCH][8], g[NCH][8], dot = 0.f;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int w = lane + 64 * WPR * c;
-    unpack8<E>(w < words ? gp[w] : u32x4{}, g[c]);
+    zero8(g[c]);
+    if (w < words) load8<EG>(a.g, row * a.D + 8 * w, g[c]);
     unpack_e4m3(w < words ? *reinterpret_cast<const u32x2*>(a.y + row * a.y_stride + 8 * w) : u32x2{}, f[c]);
     const float s = w < words ? scale_value(a.scale[row * nb + w / 16]) : 0.f;
 #pragma unroll
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256) void k_gate8(kd_gate8_args g, int64_t row0, ui
 }
 
 // da = dy b s (1 + a (1 - s)), db = dy a s, s = sigmoid(a); a and b from their 8 bits
-template <class E>
+template <class E, class EG>
 __global__ __launch_bounds__(256) void k_gate8_bwd(kd_gate8_args g, int64_t row0, uint32_t words_all, uint32_t words,
                                                    uint32_t nb) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256) void k_gate8_bwd(kd_gate8_args g, int64_t row0
   float a[8], b[8], d[8], da[8], db[8];
   unpack_e4m3(*reinterpret_cast<const u32x2*>(g.a8 + row * g.stride + w * 8), a);
   unpack_e4m3(*reinterpret_cast<const u32x2*>(g.b8 + row * g.stride + w * 8), b);
-  load8<E>(g.dy, at, d);
+  load8<EG>(g.dy, at, d);
   const float sa = scale_value(g.a_scale[row * nb + w / 16]), sb = scale_value(g.b_scale[row * nb + w / 16]);
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
@@ -341,8 +341,8 @@ int launch_norm8_bwd(const kd_norm8_bwd_args& a, hipStream_t st) {
     norm_variant<E>(a.D, [&](auto nch, auto wpr) {
       constexpr int W = decltype(wpr)::value;
       in_launches(a.rows, 64 * W, [&](int64_t r, int64_t n) {
-        hipLaunchKernelGGL((k_norm8_bwd<E, decltype(nch)::value, W>), dim3(unsigned((n * W + 3) / 4)), dim3(256), 0, st, a,
-                           r, r + n);
+        auto k = a.g_dtype == KD_F32 ? k_norm8_bwd<E, F32, decltype(nch)::value, W> : k_norm8_bwd<E, E, decltype(nch)::value, W>;
+        hipLaunchKernelGGL(k, dim3(unsigned((n * W + 3) / 4)), dim3(256), 0, st, a, r, r + n);
       });
     });
   });
@@ -363,7 +363,8 @@ int launch_gate8_bwd(const kd_gate8_args& a, hipStream_t st) {
   return by_type(a.dtype, [&](auto e) {
     in_launches(a.rows, int64_t(words), [&](int64_t r, int64_t n) {
       const uint32_t all = uint32_t(n) * words;
-      hipLaunchKernelGGL(k_gate8_bwd<decltype(e)>, dim3((all + 255) / 256), dim3(256), 0, st, a, r, all, words, nb);
+      auto k = a.dy_dtype == KD_F32 ? k_gate8_bwd<decltype(e), F32> : k_gate8_bwd<decltype(e), decltype(e)>;
+      hipLaunchKernelGGL(k, dim3((all + 255) / 256), dim3(256), 0, st, a, r, all, words, nb);
     });
   });
 }

@@ -338,6 +338,7 @@ int kd_norm8_bwd(const kd_norm8_bwd_args* a, void* stream) {
   if (a->ds != nullptr && (r = check_flat({a->ds}))) return r;
   if ((r = check_rows8(a->y, a->y_stride, a->D))) return r;
   if (a->scale == nullptr || a->rstd == nullptr) return fail(KD_ERR_INVALID, "scale and rstd are required");
+  if (a->g_dtype != a->dtype && a->g_dtype != KD_F32) return fail(KD_ERR_UNSUPPORTED, "g must be of dtype or fp32");
   r = kd::launch_norm8_bwd(*a, as_stream(stream));
   return r ? fail(r, "kernel launch failed (norm from 8 bits, backward)") : KD_OK;
 }
@@ -366,6 +367,7 @@ int kd_gate8(const kd_gate8_args* a, void* stream) {
 int kd_gate8_bwd(const kd_gate8_args* a, void* stream) {
   int r;
   if ((r = check_gate8(a, true)) || (r = check_flat({a->dy, a->da, a->db}))) return r;
+  if (a->dy_dtype != a->dtype && a->dy_dtype != KD_F32) return fail(KD_ERR_UNSUPPORTED, "dy must be of dtype or fp32");
   r = kd::launch_gate8_bwd(*a, as_stream(stream));
   return r ? fail(r, "kernel launch failed (gate from 8 bits, backward)") : KD_OK;
 }

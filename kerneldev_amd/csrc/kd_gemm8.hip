@@ -14,6 +14,8 @@
 namespace kd {
 namespace {
 
+struct F32Q {};  // fp32 results of the 8-bit product (kd_matmul8_args.fast)
+
 // Eight of an operand's 32 e4m3 values (words 2 q and 2 q + 1) as bf16
 KD_DEV u32x4 as_bf16(const i32x8& v, int q) {
   u32x4 w;
@@ -51,12 +53,12 @@ KD_DEV void tile_of(int item, int tiles_m, int tiles_n, int group, int* tm, int*
 // barrier a step.  C leaves through LDS in whole rows.
 template <class O, int BM, int BN, int WM, int WN, int PER_CU>
 struct Gemm8 {
-  static constexpr bool F = std::is_same_v<O, F32>;
+  static constexpr bool F = std::is_same_v<O, F32>, WIDE = F || std::is_same_v<O, F32Q>;
   static constexpr int NW = WM * WN, THREADS = 64 * NW, TM = BM / WM, TN = BN / WN, FA = TM / 32, FB = TN / 32;
   using TL = Tile<64>;  // 64 rows of 128 bytes, 8 KiB
   static constexpr int SLOT = (BM + BN) * 128, LOADS = SLOT / 1024 / NW;  // wave-wide 1 KiB copies a wave and step
   static constexpr int SB = 16, SROW = SB + 4;                            // blocks of K with scales in LDS
-  static constexpr int ESIZE = F ? 4 : 2, OROW = BN * ESIZE + 16;         // C in LDS
+  static constexpr int ESIZE = WIDE ? 4 : 2, OROW = BN * ESIZE + 16;         // C in LDS
   static constexpr int NBT = (BN + QB - 1) / QB;                          // B's blocks of rows in a tile
   static constexpr int POOL = 2 * SLOT > BM * OROW ? 2 * SLOT : BM * OROW;
   static constexpr int SCALES = (BM + NBT) * SROW, LDS = POOL + 2 * SCALES;
@@ -202,7 +204,7 @@ __global__ __launch_bounds__(64 * WM * WN, (PER_CU * WM * WN + 3) / 4) void k_ge
       for (int q = 0; q < 4; ++q) {  // registers 4 q ..: columns 8 q + 4 hf .. of the 32
         const f32x16& v = acc[i][j];
         uint8_t* p = s_pool + (wm * G::TM + 32 * j + c) * G::OROW + (wn * G::TN + 32 * i + 8 * q + 4 * hf) * G::ESIZE;
-        if constexpr (F) *reinterpret_cast<f32x4*>(p) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        if constexpr (G::WIDE) *reinterpret_cast<f32x4*>(p) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
         else *reinterpret_cast<u32x2*>(p) = u32x2{pack2<O>(v[4 * q], v[4 * q + 1]), pack2<O>(v[4 * q + 2], v[4 * q + 3])};
       }
   barrier_lds();
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(64 * WM * WN, (PER_CU * WM * WN + 3) / 4) void k_ge
       if (left >= PER) *reinterpret_cast<u32x4*>(q) = *reinterpret_cast<const u32x4*>(p);
       else
         for (int k = 0; k < left; ++k) {
-          if constexpr (F) reinterpret_cast<float*>(q)[k] = reinterpret_cast<const float*>(p)[k];
+          if constexpr (G::WIDE) reinterpret_cast<float*>(q)[k] = reinterpret_cast<const float*>(p)[k];
           else reinterpret_cast<uint16_t*>(q)[k] = reinterpret_cast<const uint16_t*>(p)[k];
         }
     }
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(64 * WM * WN, (PER_CU * WM * WN + 3) / 4) void k_ge
       if (n >= rows_b) continue;
       const uint8_t* p = s_pool + r * G::OROW + n * G::ESIZE;
       uint8_t* q = out + (int64_t(r) * g.ldo + n) * G::ESIZE;
-      if constexpr (F) *reinterpret_cast<float*>(q) = *reinterpret_cast<const float*>(p);
+      if constexpr (G::WIDE) *reinterpret_cast<float*>(q) = *reinterpret_cast<const float*>(p);
       else *reinterpret_cast<uint16_t*>(q) = *reinterpret_cast<const uint16_t*>(p);
     }
   }
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(64 * W) void k_gemm8_rows(kd_matmul8_args g) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (n + i < g.N) {
-        if constexpr (F) static_cast<float*>(g.out)[at + i] = v[i];
+        if constexpr (F || std::is_same_v<O, F32Q>) static_cast<float*>(g.out)[at + i] = v[i];
         else static_cast<uint16_t*>(g.out)[at + i] = uint16_t(pack2<O>(v[i], 0.f) & 0xFFFFu);
       }
   }
@@ -330,7 +332,7 @@ int go(const kd_matmul8_args& g, hipStream_t st) {
     return double((tiles + at_once - 1) / at_once) * (ends + step * double(nb));
   };
   const double large = cost(256, 256, 9.0, 1.82), mid = cost(128, 512, 4.3, 1.10), small = cost(64, 1024, 2.3, 0.84);
-  if constexpr (!std::is_same_v<O, F32>)  // (an fp32 tile of 256 x 256 does not fit the LDS on its way out)
+  if constexpr (std::is_same_v<O, BF16> || std::is_same_v<O, F16>)  // (an fp32 tile of 256 x 256 does not fit the LDS on its way out)
     if (large < mid && large < small) return go_tiles<O, 256, 256, 2, 4, 1>(g, 4, st);
   if (mid < small) return go_tiles<O, 128, 128, 4, 2, 2>(g, 8, st);
   return go_tiles<O, 64, 64, 2, 2, 4>(g, 8, st);
@@ -339,7 +341,8 @@ int go(const kd_matmul8_args& g, hipStream_t st) {
 }  // namespace
 
 int launch_matmul8(const kd_matmul8_args& g, hipStream_t st) {
-  return g.dtype == KD_BF16 ? go<BF16>(g, st) : g.dtype == KD_F16 ? go<F16>(g, st) : go<F32>(g, st);
+  if (g.dtype == KD_F32) return g.fast ? go<F32Q>(g, st) : go<F32>(g, st);
+  return g.dtype == KD_BF16 ? go<BF16>(g, st) : go<F16>(g, st);
 }
 
 }  // namespace kd

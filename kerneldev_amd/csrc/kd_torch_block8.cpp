@@ -1,27 +1,18 @@
 // The 8-bit blocks' and the embedding's operators (block_fp8.py, embed.py, which
 // declare them) from torch to the C ABI: checks of what the kernels assume,
-// allocations and launches on the current stream of the operands' device.  They
-// hold no autograd rule; the Python layer's nodes call them.
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
+// allocations and launches on the current stream of the operands' device; and
+// behind them the eager calls of the public functions, with C++ autograd nodes,
+// which return None where a call is not a plain one (the Python layer then checks it
+// and goes through its own nodes).  A step of 633 rows of 528, fp16, whose
+// kernels run for 40 us, takes 100 us through the Python nodes.
 #include <torch/library.h>
 
-#include "../../include/kdattn.h"
+#include "kd_torch.h"
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-
-void check(int status, const char* what) {
-  if (status == KD_OK) return;
-  const std::string msg = std::string(what) + ": " + kd_last_error_string();
-  TORCH_CHECK_VALUE(status != KD_ERR_INVALID && status != KD_ERR_UNSUPPORTED, msg);
-  TORCH_CHECK(false, msg, " (status ", status, ")");
-}
-
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+using namespace kdt;
+using torch::autograd::Function;
 
 int dtype_code(at::ScalarType t, bool f32) {
   if (t == at::kBFloat16) return KD_BF16;
@@ -122,7 +113,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> quant_weight8(at::TensorList ws, bool
   return {y, s, yt, st};
 }
 
-Tensor matmul8(const Tensor& a_in, const Tensor& a_scale, const Tensor& b_in, const Tensor& b_scale, at::ScalarType out_type) {
+Tensor matmul8(const Tensor& a_in, const Tensor& a_scale, const Tensor& b_in, const Tensor& b_scale, at::ScalarType out_type,
+               bool fast) {
   on_one_gpu({&a_in, &a_scale, &b_in, &b_scale});
   const Tensor a = blocks_ready(a_in), b = blocks_ready(b_in);
   const Tensor as = a_scale.contiguous(), bs = b_scale.contiguous();
@@ -133,7 +125,7 @@ Tensor matmul8(const Tensor& a_in, const Tensor& a_scale, const Tensor& b_in, co
   check_blocks(a, as, K, 1, "a"), check_blocks(b, bs, K, 128, "b");
   TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31), "M, N and K must be < 2^31");
   kd_matmul8_args g{};
-  g.dtype = dtype_code(out_type, true);
+  g.dtype = dtype_code(out_type, true), g.fast = fast;
   Tensor out = at::empty({M, N}, a.options().dtype(out_type));
   if (out.numel() == 0) return out;
   g.a = u8(a), g.b = u8(b), g.lda = a.stride(0), g.ldb = b.stride(0), g.a_scale = u8(as), g.b_scale = u8(bs);
@@ -166,7 +158,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm8(const Tensor& x_in, const OptTe
   return {sum, y, s, rstd};
 }
 
-Tensor norm8_bwd(const Tensor& g_in, const OptTensor& ds, const Tensor& y, const Tensor& scale, const Tensor& rstd) {
+Tensor norm8_bwd(const Tensor& g_in, const OptTensor& ds, const Tensor& y, const Tensor& scale, const Tensor& rstd,
+                 at::ScalarType dtype) {
   on_one_gpu({&g_in, &y, &scale, &rstd});
   TORCH_CHECK_VALUE(g_in.dim() == 2 && y.dim() == 2 && y.size(0) == g_in.size(0) && rstd.numel() == g_in.size(0) &&
                         rstd.scalar_type() == at::kFloat && rstd.is_contiguous(),
@@ -177,12 +170,12 @@ Tensor norm8_bwd(const Tensor& g_in, const OptTensor& ds, const Tensor& y, const
   Tensor d;
   if (ds) {
     on_one_gpu({&g, &*ds});
-    TORCH_CHECK_VALUE(ds->sizes() == g.sizes() && ds->scalar_type() == g.scalar_type(), "g and ds must have one shape and type");
+    TORCH_CHECK_VALUE(ds->sizes() == g.sizes() && ds->scalar_type() == dtype, "ds must have g's shape and the result's type");
     d = flat(*ds);
   }
   kd_norm8_bwd_args a{};
-  a.dtype = dtype_code(g.scalar_type(), false);
-  Tensor dx = at::empty(g.sizes(), g.options());
+  a.dtype = dtype_code(dtype, false), a.g_dtype = dtype_code(g.scalar_type(), true);
+  Tensor dx = at::empty(g.sizes(), g.options().dtype(dtype));
   a.rows = g.size(0), a.D = int32_t(g.size(1));
   if (a.rows == 0) return dx;
   a.g = g.data_ptr(), a.ds = ds ? d.data_ptr() : nullptr, a.y = u8(y), a.y_stride = y.stride(0), a.scale = u8(scale);
@@ -210,16 +203,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gate8(const Tensor& a
   return {y, ys, a8, as, b8, bs};
 }
 
-std::tuple<Tensor, Tensor> gate8_bwd(const Tensor& dy_in, const Tensor& a8, const Tensor& as, const Tensor& b8, const Tensor& bs) {
+std::tuple<Tensor, Tensor> gate8_bwd(const Tensor& dy_in, const Tensor& a8, const Tensor& as, const Tensor& b8, const Tensor& bs,
+                                     at::ScalarType dtype) {
   on_one_gpu({&dy_in, &a8, &as, &b8, &bs});
   TORCH_CHECK_VALUE(dy_in.dim() == 2 && a8.size(0) == dy_in.size(0) && b8.sizes() == a8.sizes() && b8.strides() == a8.strides(),
                     "dy, a and b must have one number of rows");
   check_blocks(a8, as, dy_in.size(1), 1, "a"), check_blocks(b8, bs, dy_in.size(1), 1, "b");
   const c10::DeviceGuard on(dy_in.device());
   const Tensor dy = flat(dy_in);
-  Tensor da = at::empty(dy.sizes(), dy.options()), db = at::empty(dy.sizes(), dy.options());
+  Tensor da = at::empty(dy.sizes(), dy.options().dtype(dtype)), db = at::empty(dy.sizes(), dy.options().dtype(dtype));
   kd_gate8_args g{};
-  g.dtype = dtype_code(dy.scalar_type(), false);
+  g.dtype = dtype_code(dtype, false), g.dy_dtype = dtype_code(dy.scalar_type(), true);
   g.rows = dy.size(0), g.H = int32_t(dy.size(1));
   if (g.rows == 0) return {da, db};
   g.dy = dy.data_ptr(), g.da = da.data_ptr(), g.db = db.data_ptr(), g.stride = a8.stride(0);
@@ -302,6 +296,284 @@ Tensor embed_grad(const Tensor& tokens_in, const Tensor& dy_in, int64_t vocab, d
   return dw;
 }
 
+// ------------------------------------------------------------ eager calls
+// The operators through the dispatcher, for cotangents of any kind
+template <class F>
+auto op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+bool half(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+bool plain_call(std::initializer_list<const Tensor*> ts) {
+  if (!plain_mode()) return false;
+  for (const Tensor* t : ts)
+    if (!plain(*t) || t->device() != (*ts.begin())->device()) return false;
+  return true;
+}
+std::vector<int64_t> with_last(const Tensor& like, int64_t last) {
+  auto shape = like.sizes().vec();
+  shape.back() = last;
+  return shape;
+}
+Tensor as_rows(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+
+bool weights_fit(const Tensor& x, at::TensorList ws) {
+  if (ws.empty() || ws.size() > 4) return false;
+  for (const Tensor& w : ws)
+    if (!plain(w) || w.dim() != 2 || w.size(1) != x.size(-1) || w.size(0) < 8 || w.size(0) % 8 != 0 ||
+        w.scalar_type() != x.scalar_type() || w.device() != x.device())
+      return false;
+  return true;
+}
+// Parts that the kernels take side by side: whole blocks, or one part
+std::vector<Tensor> stacked(at::TensorList parts, int64_t dim) {
+  bool whole = true;
+  for (size_t i = 0; i + 1 < parts.size(); ++i) whole &= parts[i].size(dim) % 128 == 0;
+  return whole ? parts.vec() : std::vector<Tensor>{at::cat(parts, dim)};
+}
+
+// The backward's products (block_fp8._backward_products): the operand's gradient
+// from the gradients' blocks and the weights', the weights' from the kept operand
+std::pair<Tensor, Tensor> backward_products(const std::vector<Tensor>& dys, const Tensor& x8, const Tensor& xs, const Tensor& wt,
+                                            const Tensor& wts, bool want_x, bool want_w, int64_t K, at::ScalarType between) {
+  static const auto quant = op<std::tuple<Tensor, Tensor>(at::TensorList)>("kdattn::quant_rows8");
+  static const auto product =
+      op<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, at::ScalarType, bool)>("kdattn::matmul8");
+  static const auto wgrad = op<Tensor(at::TensorList, const Tensor&, const Tensor&, int64_t)>("kdattn::weight_grad8");
+  const std::vector<Tensor> parts = stacked(dys, 1);
+  Tensor dx, dw;
+  if (want_x) {
+    const auto [d8, ds] = quant.call(parts);
+    dx = product.call(d8, ds, wt, wts, between, true);
+  }
+  if (want_w) dw = wgrad.call(parts, x8, xs, K);
+  return {dx, dw};
+}
+at::ScalarType between(at::ScalarType t) { return t == at::kHalf ? at::kFloat : t; }  // (block_fp8._between)
+
+// Under create_graph the results have a history that raises when it is gone back through
+variable_list once(variable_list out, const char* name, const variable_list& from) {
+  if (!at::GradMode::is_enabled()) return out;
+  bool any = false;
+  for (const Tensor& t : from) any |= t.defined() && t.requires_grad();
+  if (!any) return out;
+  variable_list given, made;
+  for (const Tensor& t : from)
+    if (t.defined()) given.push_back(t);
+  for (Tensor& t : out)
+    if (t.defined()) t = t.detach(), made.push_back(t);
+  refuse_second(made, name, given);
+  return out;
+}
+
+struct NormProjectionNode : Function<NormProjectionNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& delta, at::TensorList ws, double eps,
+                               bool want_x) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard on(x.device());
+    const int64_t K = x.size(-1);
+    const auto [s, y8, ys, rstd] = norm8(as_rows(x), delta ? OptTensor(as_rows(*delta)) : OptTensor(), eps);
+    const auto [w8, wsc, wt, wts] = quant_weight8(stacked(ws, 0), want_x);
+    const Tensor y = matmul8(y8, ys, w8, wsc, x.scalar_type(), false);
+    variable_list out;
+    if (delta) out.push_back(s.view(x.sizes()));
+    std::vector<int64_t> widths;
+    int64_t at = 0;
+    for (const Tensor& w : ws) {
+      const int64_t n = w.size(0);
+      const Tensor part = y.narrow(1, at, n);
+      out.push_back(x.dim() == 2 ? part : part.view(with_last(x, n)));
+      widths.push_back(n), at += n;
+    }
+    ctx->save_for_backward({y8, ys, rstd, wt, wts});
+    ctx->saved_data["widths"] = widths;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["type"] = int64_t(x.scalar_type());
+    ctx->saved_data["delta"] = delta.has_value();
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const bool has = ctx->saved_data["delta"].toBool();
+    const std::vector<int64_t> widths = ctx->saved_data["widths"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
+    const auto type = at::ScalarType(ctx->saved_data["type"].toInt());
+    const size_t n = widths.size(), nx = has ? 2 : 1;
+    variable_list out(2 + n + 2);
+    const bool want_x = ctx->needs_input_grad(0), want_d = has && ctx->needs_input_grad(1);
+    const Tensor dsum = has ? grads[0] : Tensor();
+    Tensor given;
+    for (size_t i = 0; i < n; ++i)
+      if (grads[i + has].defined()) given = grads[i + has];
+    if (!given.defined()) {  // the products did not reach the loss
+      if (want_x) out[0] = dsum;
+      if (want_d) out[1] = dsum;
+      return out;
+    }
+    const variable_list s = ctx->get_saved_variables();
+    const c10::DeviceGuard on(s[0].device());
+    const int64_t rows = s[0].size(0), K = shape.back();
+    std::vector<Tensor> dys;
+    bool want_w = false;
+    for (size_t i = 0; i < n; ++i) {
+      const Tensor& d = grads[i + has];
+      dys.push_back(d.defined() ? d.reshape({rows, widths[i]}) : at::zeros({rows, widths[i]}, given.options()));
+      want_w |= ctx->needs_input_grad(nx + i);
+    }
+    auto [g, dw] = backward_products(dys, s[0], s[1], s[3], s[4], want_x || want_d, want_w, K, between(type));
+    if (want_x || want_d) {
+      static const auto norm =
+          op<Tensor(const Tensor&, const OptTensor&, const Tensor&, const Tensor&, const Tensor&, at::ScalarType)>("kdattn::norm8_bwd");
+      const Tensor dx =
+          norm.call(g, dsum.defined() ? OptTensor(dsum.reshape({rows, K})) : OptTensor(), s[0], s[1], s[2], type).view(shape);
+      if (want_x) out[0] = dx;
+      if (want_d) out[1] = dx;
+    }
+    int64_t at = 0;
+    for (size_t i = 0; i < n; ++i) {
+      if (ctx->needs_input_grad(nx + i)) out[2 + i] = dw.narrow(0, at, widths[i]);
+      at += widths[i];
+    }
+    return once(std::move(out), "norm_projection", grads);
+  }
+};
+
+struct ProjectionNode : Function<ProjectionNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, bool want_x) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard on(x.device());
+    const auto [x8, xs] = quant_rows8({as_rows(x)});
+    const auto [w8, ws, wt, wts] = quant_weight8({w}, want_x);
+    const Tensor y = matmul8(x8, xs, w8, ws, x.scalar_type(), false);
+    ctx->save_for_backward({x8, xs, wt, wts});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["type"] = int64_t(x.scalar_type());
+    return x.dim() == 2 ? y : y.view(with_last(x, w.size(0)));
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const c10::DeviceGuard on(s[0].device());
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const auto [dx, dw] = backward_products({as_rows(grads[0])}, s[0], s[1], s[2], s[3], ctx->needs_input_grad(0),
+                                            ctx->needs_input_grad(1), shape.back(), at::ScalarType(ctx->saved_data["type"].toInt()));
+    return once({dx.defined() ? dx.view(shape) : dx, dw, Tensor()}, "fp8_projection", grads);
+  }
+};
+
+struct SwigluProjectionNode : Function<SwigluProjectionNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& a, const Tensor& b, const Tensor& w, bool want) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard on(a.device());
+    const auto [y8, ys, a8, as, b8, bs] = gate8(as_rows(a), as_rows(b), want);
+    const auto [w8, ws, wt, wts] = quant_weight8({w}, want);
+    const Tensor y = matmul8(y8, ys, w8, ws, a.scalar_type(), false);
+    ctx->save_for_backward({y8, ys, a8, as, b8, bs, wt, wts});
+    ctx->saved_data["shape"] = a.sizes().vec();
+    ctx->saved_data["type"] = int64_t(a.scalar_type());
+    return a.dim() == 2 ? y : y.view(with_last(a, w.size(0)));
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto gate = op<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                           at::ScalarType)>("kdattn::gate8_bwd");
+    const variable_list s = ctx->get_saved_variables();
+    const c10::DeviceGuard on(s[0].device());
+    const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
+    const auto type = at::ScalarType(ctx->saved_data["type"].toInt());
+    const bool want_a = ctx->needs_input_grad(0), want_b = ctx->needs_input_grad(1);
+    const auto [g, dw] = backward_products({as_rows(grads[0])}, s[0], s[1], s[6], s[7], want_a || want_b, ctx->needs_input_grad(2),
+                                           shape.back(), between(type));
+    Tensor da, db;
+    if (want_a || want_b) std::tie(da, db) = gate.call(g, s[2], s[3], s[4], s[5], type);
+    return once({want_a ? da.view(shape) : Tensor(), want_b ? db.view(shape) : Tensor(), dw, Tensor()}, "swiglu_projection", grads);
+  }
+};
+
+struct EmbeddingNode : Function<EmbeddingNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& tokens, double scale, int64_t padding_idx) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["pad"] = padding_idx;
+    return embed(tokens, weight, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto grad = op<Tensor(const Tensor&, const Tensor&, c10::SymInt, double, int64_t)>("kdattn::embed_grad");
+    const Tensor dw = grad.call(ctx->get_saved_variables()[0], grads[0], ctx->saved_data["vocab"].toInt(),
+                                ctx->saved_data["scale"].toDouble(), ctx->saved_data["pad"].toInt());
+    return once({dw, Tensor(), Tensor(), Tensor()}, "embedding", grads);
+  }
+};
+
+bool wants(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+pybind11::object eager_quantize_rows(const Tensor& x) {
+  if (!plain_call({&x}) || x.dim() < 1 || x.numel() == 0 || x.size(-1) % 16 != 0 || !(half(x) || x.scalar_type() == at::kFloat))
+    return pybind11::none();
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto [y, s] = quant_rows8({as_rows(x)});
+  return pybind11::make_tuple(x.dim() == 2 ? y : y.view(x.sizes()), x.dim() == 2 ? s : s.view(with_last(x, s.size(1))));
+}
+
+pybind11::object eager_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, at::ScalarType type) {
+  if (!plain_call({&a, &a_scale, &b, &b_scale}) || a.dim() < 1 || b.dim() != 2 || a.numel() == 0 || b.numel() == 0 ||
+      a.size(-1) % 16 != 0 || a.size(-1) != b.size(1) || a.scalar_type() != at::kFloat8_e4m3fn ||
+      b.scalar_type() != at::kFloat8_e4m3fn || a_scale.scalar_type() != at::kFloat8_e8m0fnu ||
+      b_scale.scalar_type() != at::kFloat8_e8m0fnu || a_scale.dim() != a.dim() || b_scale.dim() != 2 ||
+      a_scale.size(-1) != blocks(a.size(-1)) || a_scale.sizes().slice(0, a.dim() - 1) != a.sizes().slice(0, a.dim() - 1) ||
+      b_scale.size(1) != a_scale.size(-1) || b_scale.size(0) != blocks(b.size(0)) ||
+      !(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat))
+    return pybind11::none();
+  at::AutoDispatchBelowADInplaceOrView below;
+  const Tensor y = matmul8(as_rows(a), as_rows(a_scale), b, b_scale, type, false);
+  return pybind11::cast(a.dim() == 2 ? y : y.view(with_last(a, b.size(0))));
+}
+
+bool norm_fits(const Tensor& x, const OptTensor& delta, int64_t of) {
+  return plain_call({&x}) && half(x) && x.dim() >= 1 && x.numel() > 0 && x.size(-1) % of == 0 && x.size(-1) <= 8192 &&
+         (!delta || (plain(*delta) && delta->sizes() == x.sizes() && delta->scalar_type() == x.scalar_type() &&
+                     delta->device() == x.device()));
+}
+
+pybind11::object eager_norm(const Tensor& x, const OptTensor& delta, double eps) {
+  if (!norm_fits(x, delta, 16)) return pybind11::none();
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto [s, y, scale, rstd] = norm8(as_rows(x), delta ? OptTensor(as_rows(*delta)) : OptTensor(), eps);
+  if (x.dim() == 2) return pybind11::make_tuple(delta ? s : x, y, scale);
+  return pybind11::make_tuple(delta ? s.view(x.sizes()) : x, y.view(x.sizes()), scale.view(with_last(x, scale.size(1))));
+}
+
+pybind11::object eager_norm_projection(const Tensor& x, const OptTensor& delta, const std::vector<Tensor>& ws, double eps) {
+  if (!norm_fits(x, delta, 8) || !weights_fit(x, ws)) return pybind11::none();
+  variable_list out = NormProjectionNode::apply(x, delta, at::TensorList(ws), eps, wants(x) || (delta && wants(*delta)));
+  if (!delta) out.insert(out.begin(), x);
+  return pybind11::cast(out);
+}
+
+pybind11::object eager_projection(const Tensor& x, const Tensor& w) {
+  if (!plain_call({&x}) || !half(x) || x.dim() < 1 || x.numel() == 0 || x.size(-1) % 8 != 0 || !weights_fit(x, w)) return pybind11::none();
+  return pybind11::cast(ProjectionNode::apply(x, w, wants(x)));
+}
+
+pybind11::object eager_swiglu_projection(const Tensor& a, const Tensor& b, const Tensor& w) {
+  if (!plain_call({&a, &b}) || !half(a) || a.dim() < 1 || a.numel() == 0 || a.size(-1) % 8 != 0 || b.sizes() != a.sizes() ||
+      b.scalar_type() != a.scalar_type() || !weights_fit(a, w))
+    return pybind11::none();
+  return pybind11::cast(SwigluProjectionNode::apply(a, b, w, wants(a) || wants(b)));
+}
+
+pybind11::object eager_embedding(const Tensor& tokens, const Tensor& weight, double scale, std::optional<int64_t> padding_idx) {
+  if (!plain_call({&weight, &tokens}) || weight.dim() != 2 || weight.numel() == 0 || tokens.numel() == 0 ||
+      !(half(weight) || weight.scalar_type() == at::kFloat) ||
+      !(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt))
+    return pybind11::none();
+  const int64_t V = weight.size(0);
+  int64_t pad = -1;
+  if (padding_idx) {
+    if (*padding_idx < -V || *padding_idx >= V) return pybind11::none();
+    pad = *padding_idx < 0 ? *padding_idx + V : *padding_idx;
+  }
+  return pybind11::cast(EmbeddingNode::apply(weight, tokens, scale, pad));
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(kdattn, CUDA, m) {
@@ -316,3 +588,15 @@ TORCH_LIBRARY_IMPL(kdattn, CUDA, m) {
   m.impl("embed", embed);
   m.impl("embed_grad", embed_grad);
 }
+
+namespace kdt {
+void bind_block8(pybind11::module& m) {
+  m.def("quantize_rows", torch::wrap_pybind_function(eager_quantize_rows));
+  m.def("fp8_matmul", torch::wrap_pybind_function(eager_matmul));
+  m.def("add_rms_norm_fp8", torch::wrap_pybind_function(eager_norm));
+  m.def("norm_projection", torch::wrap_pybind_function(eager_norm_projection));
+  m.def("fp8_projection", torch::wrap_pybind_function(eager_projection));
+  m.def("swiglu_projection", torch::wrap_pybind_function(eager_swiglu_projection));
+  m.def("embedding", torch::wrap_pybind_function(eager_embedding));
+}
+}  // namespace kdt

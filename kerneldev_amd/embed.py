@@ -47,6 +47,8 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     ``tokens`` are int64 or int32 of any shape on the weight's GPU.  A token outside ``0 .. V - 1`` reads nothing: its
     row is NaN, and it takes no part in the gradient.  ``padding_idx`` (negative: from the end) names a token whose row of the
     gradient stays zero; it is looked up like any other."""
+    if _lib.eager(tokens, weight) and (y := _lib.native().embedding(tokens, weight, scale, padding_idx)) is not None:
+        return y
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"weight must be [V, D], got {tuple(weight.shape)}")
     if weight.dtype not in (torch.bfloat16, torch.float16, torch.float32):

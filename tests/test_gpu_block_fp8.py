@@ -25,6 +25,14 @@ TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 0.0}
 HALF = [torch.bfloat16, torch.float16]
 
 
+@pytest.fixture(params=["native", "python"])
+def route(request, monkeypatch):
+    """The C++ nodes of plain eager calls, and the Python ones that traced and transformed calls take."""
+    if request.param == "python":
+        monkeypatch.setattr(kd._lib, "eager", lambda *_: False)
+    return request.param
+
+
 def _gen(seed):
     return torch.Generator("cpu").manual_seed(seed)
 
@@ -113,7 +121,7 @@ def test_every_16_bit_pattern_and_the_edges_of_the_scale(dev):
     _same_blocks(kd.quantize_weight(x[:24].contiguous()), x[:24], 128)
 
 
-def test_strided_and_empty_operands(dev):
+def test_strided_and_empty_operands(dev, route):
     x = _data((6, 40, 3, 64), torch.bfloat16, dev, 3)
     for v in (x[:, :, 1], x.transpose(1, 2)[..., :48], x[..., 8:24], x[:, 3:4, 2, :16], x.reshape(-1)[1:1 + 16 * 9].view(9, 16)):
         a, b = kd.quantize_rows(v), kd.quantize_rows(v.contiguous())
@@ -132,7 +140,7 @@ def test_strided_and_empty_operands(dev):
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 2048, 768), (2, 130, 144), (17, 262, 768), (33, 64, 4096), (64, 129, 256),
                                    (127, 128, 128), (129, 127, 272), (300, 1000, 528), (513, 768, 2304), (1024, 1536, 640)])
-def test_fp8_matmul(dev, m, n, k, out):
+def test_fp8_matmul(dev, route, m, n, k, out):
     a, b = kd.quantize_rows(_data((m, k), torch.bfloat16, dev, m + k)), kd.quantize_weight(_data((n, k), torch.bfloat16, dev, n + k, 0.02))
     got = kd.fp8_matmul(a, b, out)
     x, w = _values(a), _values(b, 128)
@@ -165,7 +173,7 @@ def test_fp8_matmul_not_a_number_stays_in_its_row_and_column(dev):
     assert torch.equal(y.isnan(), bad)
 
 
-def test_fp8_matmul_forms(dev):
+def test_fp8_matmul_forms(dev, route):
     """Leading dimensions, rows apart in memory, unaligned bases: the same bits."""
     a, b = kd.quantize_rows(_data((4, 9, 272), torch.bfloat16, dev, 5)), kd.quantize_weight(_data((100, 272), torch.bfloat16, dev, 6))
     y = kd.fp8_matmul(a, b)
@@ -202,7 +210,7 @@ def _rounded_blocks(got, want, rel):
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("shape", [(1, 16), (1, 768), (3, 5, 528), (9, 512), (7, 1040), (2, 2048), (5, 2064), (3, 5120), (2, 8192)])
-def test_add_rms_norm_fp8(dev, shape, dtype):
+def test_add_rms_norm_fp8(dev, route, shape, dtype):
     """fp32 sum of D squares: a lane adds at most 128 (D <= 8192), the rest in a tree of 8: 2^-24 (136) on the sum, half
     of it on its root; mean, root, division and product 2^-23 each: less than 2^-16."""
     x, d = _data(shape, dtype, dev, sum(shape)), _data(shape, dtype, dev, sum(shape) + 1)
@@ -256,7 +264,7 @@ STEPS = [(1, 8, 8), (1, 768, 768), (63, 136, 128), (65, 1000, 528), (200, 264, 5
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("m,n,k", STEPS)
-def test_fp8_projection(dev, m, n, k, dtype):
+def test_fp8_projection(dev, route, m, n, k, dtype):
     x, w = _data((m, k), dtype, dev, m).requires_grad_(True), _data((n, k), dtype, dev, n, 0.02).requires_grad_(True)
     dy = _data((m, n), dtype, dev, k, 0.01)
     y = kd.fp8_projection(x, w)
@@ -273,7 +281,7 @@ def test_fp8_projection(dev, m, n, k, dtype):
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("m,ns,k", [(1, (8,), 8), (5, (128, 256, 72), 264), (66, (40, 64), 2064), (700, (256, 256, 256), 256),
                                     (2049, (512, 128, 128, 8), 768), (130, (96, 96, 96), 1024), (3, (16,), 8192)])
-def test_norm_projection(dev, m, ns, k, dtype):
+def test_norm_projection(dev, route, m, ns, k, dtype):
     """The gradient of the rows: g rounded to 16 bits (u), then dx = ds + r (g - y mean(g y)) in fp32, rounded (u)."""
     x, d = _data((m, k), dtype, dev, m).requires_grad_(True), _data((m, k), dtype, dev, m + 1).requires_grad_(True)
     ws = [_data((n, k), dtype, dev, n + i, 0.02).requires_grad_(True) for i, n in enumerate(ns)]
@@ -300,7 +308,7 @@ def test_norm_projection(dev, m, ns, k, dtype):
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("m,n,k", STEPS)
-def test_swiglu_projection(dev, m, n, k, dtype):
+def test_swiglu_projection(dev, route, m, n, k, dtype):
     a, b = _data((m, k), dtype, dev, m).requires_grad_(True), _data((m, k), dtype, dev, m + 1).requires_grad_(True)
     w, dy = _data((n, k), dtype, dev, n, 0.02).requires_grad_(True), _data((m, n), dtype, dev, k, 0.01)
     y = kd.swiglu_projection(a, b, w)
@@ -353,7 +361,7 @@ def test_differences(dev):
         assert (f(x, w.detach() + e) - f(x, w.detach() - e)) / 2 == dw[i, j].item()
 
 
-def test_parts_of_the_gradient(dev):
+def test_parts_of_the_gradient(dev, route):
     """Operands that want no gradient, outputs that reach no loss, gradients of unusual layout."""
     x, d = (_data((2, 9, 256), torch.bfloat16, dev, i).requires_grad_(True) for i in (1, 2))
     ws = [_data((128, 256), torch.bfloat16, dev, i, 0.02).requires_grad_(True) for i in (3, 4, 5)]
@@ -366,8 +374,9 @@ def test_parts_of_the_gradient(dev):
     assert torch.equal(torch.autograd.grad(q, ws[0], dt, retain_graph=True)[0],
                        torch.autograd.grad(q, ws[0], dt.contiguous(), retain_graph=True)[0])
     g, = torch.autograd.grad(q.float().square().sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
+    with pytest.raises(RuntimeError, match="once_differentiable|no autograd formula"):
         g.float().sum().backward()
+    assert ("CppFunction" in type(q.grad_fn).__name__) == (route == "native")
     # frozen weights, frozen rows
     y = kd.fp8_projection(x, ws[0].detach())
     gx, = torch.autograd.grad(y, x, torch.ones_like(y))
@@ -433,7 +442,7 @@ def _mlp(x, d, w1, w3, w2):
     return s + kd.swiglu_projection(a, b, w2)
 
 
-def test_a_run_of_them_captured_and_on_another_stream(dev):
+def test_a_run_of_them_captured_and_on_another_stream(dev, route):
     x, d = (_data((300, 256), torch.bfloat16, dev, i).requires_grad_(True) for i in (1, 2))
     w1, w3 = (_data((384, 256), torch.bfloat16, dev, i, 0.05).requires_grad_(True) for i in (3, 4))
     w2, dy = _data((256, 384), torch.bfloat16, dev, 5, 0.05).requires_grad_(True), _data((300, 256), torch.bfloat16, dev, 6)

@@ -14,6 +14,13 @@ U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 **
 TYPES = list(U)
 
 
+@pytest.fixture(params=["native", "python"])
+def route(request, monkeypatch):
+    if request.param == "python":
+        monkeypatch.setattr(kd._lib, "eager", lambda *_: False)
+    return request.param
+
+
 def _case(tokens, vocab, dim, dtype, dev, seed=0):
     g = torch.Generator("cpu").manual_seed(seed)
     w = torch.randn(vocab, dim, generator=g).to(dtype).to(dev).requires_grad_(True)
@@ -58,7 +65,7 @@ def test_runs_of_equal_tokens(dev, dtype):
         _check(t, w, dy, 0.5)
 
 
-def test_shapes_strides_and_the_outside(dev):
+def test_shapes_strides_and_the_outside(dev, route):
     g = torch.Generator("cpu").manual_seed(1)
     tokens = torch.randint(0, 50, (6, 37, 2), generator=g)
     t, w, dy = _case(tokens, 50, 24, torch.bfloat16, dev)
@@ -78,6 +85,10 @@ def test_shapes_strides_and_the_outside(dev):
     odd = torch.randn(51 * 24 + 1, device=dev).bfloat16()[1:].view(51, 24).requires_grad_(True)  # a base of 2 bytes
     _check(t, odd, dy)
     y = kd.embedding(t, w)
+    assert ("CppFunction" in type(y.grad_fn).__name__) == (route == "native")
+    g, = torch.autograd.grad((y * w[0]).float().sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|no autograd formula"):
+        g.float().sum().backward()
     s, = torch.autograd.grad(y.sum(), w)  # an expanded gradient
     assert torch.equal(s, torch.autograd.grad(kd.embedding(t, w), w, torch.ones_like(y))[0])
 
