@@ -88,7 +88,7 @@ def build_native(verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=len(objs)) as ex:
         list(ex.map(lambda so: _run(["g++", *flags, "-c", so[0], "-o", so[1]]), zip(NATIVE_SRCS, objs)))
     _run(["g++", "-shared", *objs, "-o", tmp, f"-L{PKG}", "-lkdattn", *libdirs, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
-          "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+          "-ltorch_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, NATIVE)
     if verbose:
         print(f"built {NATIVE}")

@@ -59,8 +59,36 @@ KD_DEV float scale_value(uint32_t byte) {  // 2^(byte - 127); 2^-127 is subnorma
 }
 KD_DEV float scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }  // byte <= 253
 
-// Eight values as e4m3 bytes under the scale whose inverse is inv (round to
-// nearest even; scaled values are at most 448)
+// Eight finite values as e4m3 bytes under the scale (round to nearest even; scaled
+// values are at most 448).  The conversions divide by the power of two themselves.
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+KD_DEV u32x2 pack_finite(const float (&f)[8], float scale) {
+  u32x2 w;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    s16x2 r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(s16x2{}, f[4 * k], f[4 * k + 1], scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, f[4 * k + 2], f[4 * k + 3], scale, true);
+    w[k] = __builtin_bit_cast(uint32_t, r);
+  }
+  return w;
+}
+// Bits of max |f|, NaN and infinities among them (0x7F800000 and above)
+KD_DEV uint32_t any_max(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  return m;
+}
+// the same of eight bf16 or fp16, as a 16-bit number
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+KD_DEV uint32_t any_max(const u32x4& v) {
+  u16x2 m = __builtin_bit_cast(u16x2, v[0] & 0x7FFF7FFFu);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7FFF7FFFu));
+  return max(uint32_t(m[0]), uint32_t(m[1]));
+}
+
+// Eight values as e4m3 bytes under the scale whose inverse is inv, NaN where they are not finite
 KD_DEV u32x2 pack_e4m3(const float (&f)[8], float inv) {
   float g[8];
 #pragma unroll

@@ -31,21 +31,53 @@ KD_DEV void zero8(float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = 0.f;
 }
 
-// x[p], p < 4 (an index into a kernel argument would copy the array to scratch memory)
-template <class T>
-KD_DEV T pick(const T (&x)[4], int p) {
-  return p == 0 ? x[0] : p == 1 ? x[1] : p == 2 ? x[2] : x[3];
+// The scale's byte and the e4m3 bytes of the lane's 8 values, the block's lanes (a
+// DPP row) together.  Blocks that hold a NaN or an infinity take the longer way, and
+// with them their wave.
+KD_DEV u32x2 quantise(const float (&f)[8], uint32_t* byte) {
+  uint32_t m = row16_max(any_max(f));
+  if (__builtin_amdgcn_ballot_w64(m >= 0x7F800000u) != 0) {
+    *byte = scale_byte(row16_max(finite_max(f)));
+    return pack_e4m3(f, scale_inverse(*byte));
+  }
+  *byte = scale_byte(m);
+  return pack_finite(f, scale_value(*byte));
+}
+template <class E>
+KD_DEV u32x2 quantise(const u32x4& v, uint32_t* byte) {
+  constexpr bool B = std::is_same_v<E, BF16>;
+  const uint32_t m = row16_max(any_max(v));
+  float f[8];
+  unpack8<E>(v, f);
+  if (__builtin_amdgcn_ballot_w64(m >= (B ? 0x7F80u : 0x7C00u)) != 0) {
+    *byte = scale_byte(row16_max(finite_max(f)));
+    return pack_e4m3(f, scale_inverse(*byte));
+  }
+  *byte = scale_byte(B ? m << 16 : __float_as_uint(to_f32<E>(uint16_t(m))));
+  return pack_finite(f, scale_value(*byte));
 }
 
 // The lane's 8 values at column col of row `row` as part of their block, and
 // the block's scale byte by its first lane.  All lanes of a DPP row call it
 // together; those at or behind column `cols` hold zeros.
+KD_DEV void store_bytes(const u32x2& w, uint32_t byte, uint8_t* y, int64_t y_stride, uint8_t* scale, int64_t nb, int64_t row,
+                        int col, int cols) {
+  if (col < (cols + 15) / 16 * 16)  // (the row's 16-byte words whole: zeros behind its end)
+    *reinterpret_cast<u32x2*>(y + row * y_stride + col) = w;
+  if ((threadIdx.x & 15) == 0 && col < cols) scale[row * nb + col / QB] = uint8_t(byte);
+}
 KD_DEV void store_block(const float (&f)[8], uint8_t* y, int64_t y_stride, uint8_t* scale, int64_t nb, int64_t row,
                         int col, int cols) {
-  const uint32_t b = scale_byte(row16_max(finite_max(f)));
-  if (col < y_stride && col < (cols + 15) / 16 * 16)  // (the row's 16-byte words whole: zeros behind its end)
-    *reinterpret_cast<u32x2*>(y + row * y_stride + col) = pack_e4m3(f, scale_inverse(b));
-  if ((threadIdx.x & 15) == 0 && col < cols) scale[row * nb + col / QB] = uint8_t(b);
+  uint32_t b;
+  const u32x2 w = quantise(f, &b);
+  store_bytes(w, b, y, y_stride, scale, nb, row, col, cols);
+}
+template <class E>
+KD_DEV void store_block(const u32x4& v, uint8_t* y, int64_t y_stride, uint8_t* scale, int64_t nb, int64_t row, int col,
+                        int cols) {
+  uint32_t b;
+  const u32x2 w = quantise<E>(v, &b);
+  store_bytes(w, b, y, y_stride, scale, nb, row, col, cols);
 }
 
 template <class E>
@@ -54,40 +86,59 @@ __global__ __launch_bounds__(256) void k_quant_rows(kd_rows8_args a, int64_t row
   const uint32_t r = blk / nb, kb = blk - r * nb;
   const int64_t row = row0 + r;
   const int col = int(kb) * QB + int(threadIdx.x & 15) * 8;
-  float f[8];
-  zero8(f);
+  if (blk >= blocks) return;  // (whole DPP rows)
   // the part that holds the column (parts before the last end on a block's edge)
-  int p = 0, c = col;
+  const void* x = a.x[0];
+  int64_t stride = a.x_stride[0];
+  int c = col, cols = a.cols[0];
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (p == i && i + 1 < a.n && c >= a.cols[i]) c -= a.cols[i], p = i + 1;
-  if (blk < blocks && col < a.total) load8<E>(pick(a.x, p), row * pick(a.x_stride, p) + c, f);
-  if (blk < blocks) store_block(f, a.y, a.y_stride, a.scale, nb, row, col, a.total);
+  for (int i = 1; i < 4; ++i)
+    if (i < a.n && c >= cols) c -= cols, x = a.x[i], stride = a.x_stride[i], cols = a.cols[i];
+  const int64_t at = row * stride + c;
+  if constexpr (std::is_same_v<E, F32>) {
+    float f[8];
+    zero8(f);
+    if (col < a.total) load8<F32>(x, at, f);
+    store_block(f, a.y, a.y_stride, a.scale, nb, row, col, a.total);
+  } else {
+    u32x4 v{};
+    if (col < a.total) v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + at);
+    store_block<E>(v, a.y, a.y_stride, a.scale, nb, row, col, a.total);
+  }
 }
 
-// A workgroup a block of 128 x 128: 16 threads a row, 8 rows a thread; the
-// bytes go out as they are, and through LDS transposed.  Byte (r, c) lies at
-// row c of the transposed tile, whose rows are 132 bytes so that 16 of them
-// start in different banks.
+// The bytes of a 4 x 4 block turned over: word j of the result holds byte j of the four words
+KD_DEV void turn4(const uint32_t (&r)[4], uint32_t (&c)[4]) {
+  const uint32_t t0 = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u), t1 = __builtin_amdgcn_perm(r[3], r[2], 0x05010400u),
+                 t2 = __builtin_amdgcn_perm(r[1], r[0], 0x07030602u), t3 = __builtin_amdgcn_perm(r[3], r[2], 0x07030602u);
+  c[0] = __builtin_amdgcn_perm(t1, t0, 0x05040100u), c[1] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+  c[2] = __builtin_amdgcn_perm(t3, t2, 0x05040100u), c[3] = __builtin_amdgcn_perm(t3, t2, 0x07060302u);
+}
+
+// A workgroup a block of 128 x 128, a thread 8 rows of 8 columns: the bytes go out
+// as they are and, turned over in registers, transposed.  Latency bounds it (a
+// model's weight is some hundred blocks): one round of loads, one exchange of the
+// maximum (16384 tokens' q, k and v, 2304 x 768: 4 us; through LDS, byte by byte, 10).
 template <class E>
 __global__ __launch_bounds__(256) void k_quant_weight(kd_weight8_args a, uint32_t kblocks, uint32_t nblocks) {
   __shared__ uint32_t s_max[4];
-  __shared__ __attribute__((aligned(16))) uint8_t s_t[QB * 132];
   const int tid = threadIdx.x, nb = blockIdx.x / kblocks, kb = blockIdx.x - nb * kblocks;
-  int part = 0, first = nb * QB;  // rows of the part that holds this block (parts before the last: whole blocks)
+  const void* src = a.w[0];  // the part that holds this block (parts before the last: whole blocks)
+  int64_t stride = a.w_stride[0];
+  int first = nb * QB, height = a.rows[0];
 #pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (part == i && i + 1 < a.n && first >= a.rows[i]) first -= a.rows[i], part = i + 1;
-  const int rows = min(QB, pick(a.rows, part) - first), col = kb * QB + (tid & 15) * 8;
+  for (int i = 1; i < 4; ++i)
+    if (i < a.n && first >= height) first -= height, src = a.w[i], stride = a.w_stride[i], height = a.rows[i];
+  const int rows = min(QB, height - first), r0 = (tid >> 4) * 8, col = kb * QB + (tid & 15) * 8;
   float f[8][8];
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = (tid >> 4) + 16 * i;
     zero8(f[i]);
-    if (r < rows && col < a.K) load8<E>(pick(a.w, part), int64_t(first + r) * pick(a.w_stride, part) + col, f[i]);
-    m = max(m, finite_max(f[i]));
+    if (r0 + i < rows && col < a.K) load8<E>(src, int64_t(first + r0 + i) * stride + col, f[i]);
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, finite_max(f[i]));
   m = row16_max(m);
   m = max(m, uint32_t(__shfl_xor(int(m), 16, 64)));
   m = max(m, uint32_t(__shfl_xor(int(m), 32, 64)));
@@ -100,38 +151,35 @@ __global__ __launch_bounds__(256) void k_quant_weight(kd_weight8_args a, uint32_
     a.scale[int64_t(nb) * kblocks + kb] = uint8_t(b);
     if (a.scale_t != nullptr) a.scale_t[int64_t(kb) * nblocks + nb] = uint8_t(b);
   }
+  u32x2 w[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = (tid >> 4) + 16 * i;
-    const u32x2 w = pack_e4m3(f[i], inv);
-    if (r < rows && col < (a.K + 15) / 16 * 16 && col < a.y_stride)
-      *reinterpret_cast<u32x2*>(a.y + (int64_t(nb) * QB + r) * a.y_stride + col) = w;
-    if (a.yt != nullptr) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) s_t[((tid & 15) * 8 + k) * 132 + r] = uint8_t(w[k >> 2] >> (8 * (k & 3)));
-    }
+    w[i] = pack_e4m3(f[i], inv);
+    if (r0 + i < rows && col < (a.K + 15) / 16 * 16)
+      *reinterpret_cast<u32x2*>(a.y + (int64_t(nb) * QB + r0 + i) * a.y_stride + col) = w[i];
   }
-  if (a.yt == nullptr) return;  // (uniform)
-  __syncthreads();
-  const int total16 = (a.total + 15) / 16 * 16;
+  if (a.yt == nullptr || nb * QB + r0 >= (a.total + 15) / 16 * 16) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int k = (tid >> 4) + 16 * i, n = (tid & 15) * 8;
-    if (kb * QB + k < a.K && nb * QB + n < total16 && nb * QB + n < a.yt_stride) {
-      const uint32_t* p = reinterpret_cast<const uint32_t*>(s_t + k * 132 + n);
-      *reinterpret_cast<u32x2*>(a.yt + int64_t(kb * QB + k) * a.yt_stride + nb * QB + n) = u32x2{p[0], p[1]};
-    }
+  for (int h = 0; h < 2; ++h) {
+    uint32_t lo[4], hi[4];
+    turn4({w[0][h], w[1][h], w[2][h], w[3][h]}, lo);
+    turn4({w[4][h], w[5][h], w[6][h], w[7][h]}, hi);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + 4 * h + j < a.K)
+        *reinterpret_cast<u32x2*>(a.yt + int64_t(col + 4 * h + j) * a.yt_stride + nb * QB + r0) = u32x2{lo[j], hi[j]};
   }
 }
 
 // Sum over the WPR waves that share a row
-template <int WPR>
-KD_DEV float row_sum(float x, float* s_part) {
-  x = wave_sum(x);
+template <int WPR, class T>
+KD_DEV T row_sum(T x, T* s_part) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
   if constexpr (WPR > 1) {
     if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = x;
     __syncthreads();
-    x = 0.f;
+    x = 0;
 #pragma unroll
     for (int i = 0; i < WPR; ++i) x += s_part[i];
   }
@@ -140,17 +188,22 @@ KD_DEV float row_sum(float x, float* s_part) {
 
 // s = x + delta rounded to its type (what the next layer adds to), y = s
 // rsqrt(mean(s^2) + eps) in 8 bits.  WPR waves a row, lane l of the row holds the
-// 8-value words l, l + 64 WPR, ...: the row stays in registers.
+// 8-value words l, l + 64 WPR, ...: the row stays in registers.  The sum of
+// squares and its root are formed in 64 bits and y = s r with r as two floats: y is
+// the exact value's fp32 rounding, nearly always, and its 8 bits those of the exact
+// value (rounded from an fp32 root, some ten of 10^7 were not).  Memory bounds it all
+// the same.
 template <class E, int NCH, int WPR>
 __global__ __launch_bounds__(256) void k_norm8(kd_norm8_args a, int64_t row0, int64_t end) {
-  __shared__ float s_part[4];
+  __shared__ double s_part[4];
   const int lane = threadIdx.x & (64 * WPR - 1);
   const int64_t at = row0 + int64_t(blockIdx.x) * (4 / WPR) + threadIdx.x / (64 * WPR);
   const int64_t row = at < end ? at : end - 1;  // (a wave without a row follows the last, storing nothing)
   const bool live = at < end;
   const int words = a.D / 8;
   const u32x4 *x = static_cast<const u32x4*>(a.x) + row * words, *d = static_cast<const u32x4*>(a.delta) + row * words;
-  float f[NCH][8], sum = 0.f;
+  float f[NCH][8];
+  double sum = 0.0;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int w = lane + 64 * WPR * c;
@@ -172,14 +225,17 @@ __global__ __launch_bounds__(256) void k_norm8(kd_norm8_args a, int64_t row0, in
 #pragma unroll
   for (int c = 0; c < NCH; ++c)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(f[c][i], f[c][i], sum);
-  const float r = 1.f / sqrtf(row_sum<WPR>(sum, s_part) / float(a.D) + a.eps);
+    for (int i = 0; i < 8; ++i) sum = __builtin_fma(double(f[c][i]), double(f[c][i]), sum);
+  const double v = row_sum<WPR>(sum, s_part) / double(a.D) + double(a.eps);
+  const double g = double(1.f / sqrtf(float(v))), root = g * (1.5 - 0.5 * v * g * g);  // one step of Newton's
+  const bool fine = g > 0.0 && g < double(__builtin_inff());                           // (else 0, infinite or NaN, as g is)
+  const float r = fine ? float(root) : float(g), rest = fine ? float(root - double(r)) : 0.f;
   if (live && lane == 0 && a.rstd != nullptr) a.rstd[row] = r;
   const int64_t nb = (a.D + QB - 1) / QB;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[c][i] *= r;
+    for (int i = 0; i < 8; ++i) f[c][i] = __builtin_fmaf(f[c][i], r, f[c][i] * rest);
     if (live) store_block(f[c], a.y, a.y_stride, a.scale, nb, row, (lane + 64 * WPR * c) * 8, a.D);
   }
 }
@@ -222,7 +278,8 @@ __global__ __launch_bounds__(256) void k_norm8_bwd(kd_norm8_bwd_args a, int64_t 
   }
 }
 
-KD_DEV float sigmoid8(float x) { return 1.f / (1.f + fast_exp2(x * -1.4426950408889634f)); }
+// (the reciprocal within 1 ulp; of infinity 0)
+KD_DEV float sigmoid8(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(x * -1.4426950408889634f)); }
 
 // y = silu(a) b, and a and b themselves, in 8 bits
 template <class E>
@@ -231,16 +288,20 @@ __global__ __launch_bounds__(256) void k_gate8(kd_gate8_args g, int64_t row0, ui
   const uint32_t r = blk / nb, kb = blk - r * nb;
   const int64_t row = row0 + r;
   const int col = int(kb) * QB + int(threadIdx.x & 15) * 8;
+  if (blk >= blocks) return;  // (whole DPP rows)
+  u32x4 va{}, vb{};
+  if (col < g.H) {
+    va = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(g.a) + row * g.a_stride + col);
+    vb = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(g.b) + row * g.b_stride + col);
+  }
   float a[8], b[8], y[8];
-  zero8(a), zero8(b);
-  if (blk < blocks && col < g.H) load8<E>(g.a, row * g.a_stride + col, a), load8<E>(g.b, row * g.b_stride + col, b);
+  unpack8<E>(va, a), unpack8<E>(vb, b);
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = a[i] * sigmoid8(a[i]) * b[i];
-  if (blk >= blocks) return;  // (whole DPP rows)
   store_block(y, g.y8, g.stride, g.y_scale, nb, row, col, g.H);
   if (g.a8 == nullptr) return;
-  store_block(a, g.a8, g.stride, g.a_scale, nb, row, col, g.H);
-  store_block(b, g.b8, g.stride, g.b_scale, nb, row, col, g.H);
+  store_block<E>(va, g.a8, g.stride, g.a_scale, nb, row, col, g.H);
+  store_block<E>(vb, g.b8, g.stride, g.b_scale, nb, row, col, g.H);
 }
 
 // da = dy b s (1 + a (1 - s)), db = dy a s, s = sigmoid(a); a and b from their 8 bits

@@ -5,8 +5,8 @@
 // the token, stable, so that equal tokens become a run whose rows are added in
 // fp32 in the order of their positions: no atomics, and a result that does not
 // change from run to run.  A row of dy is read once.  The sorted list is cut into
-// chunks of 32 positions, one wave a chunk and 256 columns, so that a token that
-// fills the batch costs what 32-row runs cost; runs that cross a chunk's edge
+// chunks of 16 positions, one wave a chunk and 256 columns, eight rows in flight at
+// once, so that a token that fills the batch costs what short runs cost; runs that cross a chunk's edge
 // leave partial sums, which a last launch adds in order.  A token outside the
 // vocabulary reads nothing: its row of y is NaN and it takes no part in dW.
 #include <algorithm>
@@ -17,9 +17,9 @@
 namespace kd {
 namespace {
 
-constexpr int CHUNK = 32;       // sorted positions a wave adds
+constexpr int CHUNK = 16;       // sorted positions a wave adds
 constexpr int SORT_T = 1024;    // threads of a sorting workgroup
-constexpr int SORT_N = 4096;    // positions it takes: four a thread
+constexpr int SORT_N = 1024;    // positions it takes: one a thread
 constexpr int MAX_BINS = 2048;  // a pass sorts by up to 11 bits
 constexpr int JOIN_W = 8;       // waves that share a long run's partial sums
 
@@ -46,7 +46,9 @@ KD_DEV void load_v(const void* p, int64_t at, float (&f)[V]) {
     }
   } else {
     const uint16_t* q = static_cast<const uint16_t*>(p) + at;
-    if constexpr (V == 4) {
+    if constexpr (V == 8) {
+      unpack8<E>(*reinterpret_cast<const u32x4*>(q), f);
+    } else if constexpr (V == 4) {
       const u32x2 u = *reinterpret_cast<const u32x2*>(q);
 #pragma unroll
       for (int i = 0; i < 2; ++i) f[2 * i] = to_f32<E>(uint16_t(u[i] & 0xFFFFu)), f[2 * i + 1] = to_f32<E>(uint16_t(u[i] >> 16));
@@ -73,7 +75,8 @@ KD_DEV void store_v(void* p, int64_t at, const float (&f)[V]) {
     else q[0] = f[0];
   } else {
     uint16_t* q = static_cast<uint16_t*>(p) + at;
-    if constexpr (V == 4) *reinterpret_cast<u32x2*>(q) = u32x2{pack2<E>(f[0], f[1]), pack2<E>(f[2], f[3])};
+    if constexpr (V == 8) *reinterpret_cast<u32x4*>(q) = pack8<E>(f);
+    else if constexpr (V == 4) *reinterpret_cast<u32x2*>(q) = u32x2{pack2<E>(f[0], f[1]), pack2<E>(f[2], f[3])};
     else q[0] = uint16_t(pack2<E>(f[0], 0.f) & 0xFFFFu);
   }
 }
@@ -213,10 +216,11 @@ __global__ __launch_bounds__(SORT_T) void k_sort_move(kd_embed_args a, SortPass 
       before[j] = s.hist[int64_t(blk) * bins + b];
     } else if (s.blocks > 1) {
       total[j] = 0;
+#pragma unroll 8
       for (int k = 0; k < s.blocks; ++k) {
         const uint32_t n = s.hist[int64_t(k) * bins + b];
         total[j] += n;
-        if (k < blk) before[j] += n;
+        before[j] += k < blk ? n : 0u;
       }
     }
   }
@@ -284,7 +288,9 @@ __global__ __launch_bounds__(256) void k_embed_runs(kd_embed_args a, Runs s) {
     store_v<E, V>(a.dw, int64_t(run) * a.dim + col, f);
   };
   zero();
-  for (int r0 = 0; r0 < n; r0 += 8) {
+#pragma unroll
+  for (int r0 = 0; r0 < CHUNK; r0 += 8) {
+    if (r0 >= n) break;
     float v[8][V];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -295,15 +301,16 @@ __global__ __launch_bounds__(256) void k_embed_runs(kd_embed_args a, Runs s) {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (r0 + j >= n) break;
-      const uint32_t k0 = key_of(r0 + j);
-      if (k0 != run) {
-        flush(false);
-        run = k0;
-        zero();
-      }
+      if (r0 + j < n) {
+        const uint32_t k0 = key_of(r0 + j);
+        if (k0 != run) {
+          flush(false);
+          run = k0;
+          zero();
+        }
 #pragma unroll
-      for (int k = 0; k < V; ++k) sum[k] += v[j][k];
+        for (int k = 0; k < V; ++k) sum[k] += v[j][k];
+      }
     }
   }
   flush(true);
@@ -355,6 +362,80 @@ __global__ __launch_bounds__(64 * JOIN_W) void k_embed_join(kd_embed_args a, Run
   store_v<E, V>(a.dw, int64_t(run) * a.dim + col, f);
 }
 
+// Few positions: one launch.  A workgroup takes R rows of dW, lists in order the
+// positions whose tokens lie among them, and for each row adds the listed rows of
+// dy, eight in flight; rows without a token are written as zeros.
+constexpr int SMALL_N = 512;
+template <class E, int V>
+__global__ __launch_bounds__(256) void k_embed_small(kd_embed_args a, int R) {
+  __shared__ uint32_t s_list[SMALL_N + 64];  // position << 8 | row
+  __shared__ int s_count[SMALL_N / 64 + 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = int(a.n);
+  const int64_t v0 = int64_t(blockIdx.x) * R;
+  const int rows = int(min(int64_t(R), a.vocab - v0));
+  // groups of 64 positions, two a wave
+  uint64_t found[2];
+  int row[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    const int i = (2 * wave + g) * 64 + lane;
+    const int64_t at = i < n ? int64_t(key_at(a, i)) - v0 : -1;
+    row[g] = int(at);
+    const bool in = at >= 0 && at < rows;
+    found[g] = __builtin_amdgcn_ballot_w64(in);
+    if (lane == 0) s_count[2 * wave + g] = __builtin_popcountll(found[g]);
+  }
+  __syncthreads();
+  int total = 0, before[2] = {0, 0};
+#pragma unroll
+  for (int g = 0; g < SMALL_N / 64; ++g) {
+    if (g == 2 * wave) before[0] = total;
+    if (g == 2 * wave + 1) before[1] = total;
+    total += s_count[g];
+  }
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    if ((found[g] >> lane) & 1u)
+      s_list[before[g] + __builtin_popcountll(found[g] & ((uint64_t(1) << lane) - 1u))] =
+          uint32_t((2 * wave + g) * 64 + lane) << 8 | uint32_t(row[g]);
+  __syncthreads();
+  for (int r = 0; r < rows; ++r) {
+    for (int64_t c0 = 0; c0 < a.dim; c0 += 256 * V) {
+      const int64_t col = c0 + tid * V;
+      const bool in = col < a.dim;
+      float sum[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum[k] = 0.f;
+      for (int g = 0; g < total; g += 64) {
+        const uint32_t e = g + lane < total ? s_list[g + lane] : 0xFFFFFFFFu;
+        uint64_t todo = __builtin_amdgcn_ballot_w64((e & 255u) == uint32_t(r) && g + lane < total);
+        while (todo != 0) {  // (uniform, at most 8 rounds)
+          float f[8][V];
+          int m = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[j][k] = 0.f;
+            if (todo != 0) {
+              const uint32_t p = uint32_t(__builtin_amdgcn_readlane(int(e), __builtin_ctzll(todo))) >> 8;
+              todo &= todo - 1;
+              m = j + 1;
+              if (in) load_v<E, V>(a.dy, int64_t(p) * a.dim + col, f[j]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < m)
+#pragma unroll
+              for (int k = 0; k < V; ++k) sum[k] += f[j][k];
+        }
+      }
+      scaled<V>(sum, a.scale);
+      if (in) store_v<E, V>(a.dw, (v0 + r) * a.dim + col, sum);
+    }
+  }
+}
+
 struct EmbedLayout {
   int64_t keys[2], idx[2], hist, part, total;  // bytes from the workspace's start
   int64_t chunks;
@@ -363,6 +444,10 @@ struct EmbedLayout {
 
 EmbedLayout embed_layout(int64_t n, int64_t vocab, int64_t dim) {
   EmbedLayout L{};
+  if (n <= SMALL_N) {
+    L.total = 256;  // (nothing is needed; a pointer is)
+    return L;
+  }
   int bits = 1;
   while ((int64_t(1) << bits) <= vocab) ++bits;  // keys are 0 .. vocab
   L.passes = (bits + 10) / 11;
@@ -415,18 +500,30 @@ int launch_embed(const kd_embed_args& a, hipStream_t st) {
                            uint32_t(words));
       }
     };
+    if constexpr (!std::is_same_v<E, F32>)
+      if (a.dim % 8 == 0 && by_four(a, {a.weight, a.out})) return go(int_c<8>{});
     if (by_four(a, {a.weight, a.out})) go(int_c<4>{});
     else go(int_c<1>{});
   });
 }
 
 int launch_embed_grad(const kd_embed_args& a, uint8_t* ws, hipStream_t st) {
+  if (a.n <= SMALL_N)
+    return by_type(a.dtype, [&](auto e) {
+      using E = decltype(e);
+      const int R = int(std::max<int64_t>(1, std::min<int64_t>(64, a.vocab / 1024)));
+      auto go = [&](auto v) {
+        hipLaunchKernelGGL((k_embed_small<E, decltype(v)::value>), dim3(unsigned((a.vocab + R - 1) / R)), dim3(256), 0, st, a, R);
+      };
+      if (by_four(a, {a.dy, a.dw})) go(int_c<4>{});
+      else go(int_c<1>{});
+    });
   const EmbedLayout L = embed_layout(a.n, a.vocab, a.dim);
   auto u32 = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
   const int64_t bytes = a.vocab * a.dim * (a.dtype == KD_F32 ? 4 : 2);
   SortPass s{};
   s.bits = L.bits, s.blocks = L.blocks, s.hist = u32(L.hist);
-  s.scanned = L.blocks > 16;
+  s.scanned = L.blocks > 64;
   for (int p = 0; p < L.passes; ++p) {
     s.keys = p == 0 ? nullptr : u32(L.keys[(p - 1) & 1]), s.idx = p == 0 ? nullptr : u32(L.idx[(p - 1) & 1]);
     s.keys_out = u32(L.keys[p & 1]), s.idx_out = u32(L.idx[p & 1]);

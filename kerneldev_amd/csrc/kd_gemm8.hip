@@ -334,7 +334,10 @@ int go(const kd_matmul8_args& g, hipStream_t st) {
   const double large = cost(256, 256, 9.0, 1.82), mid = cost(128, 512, 4.3, 1.10), small = cost(64, 1024, 2.3, 0.84);
   if constexpr (std::is_same_v<O, BF16> || std::is_same_v<O, F16>)  // (an fp32 tile of 256 x 256 does not fit the LDS on its way out)
     if (large < mid && large < small) return go_tiles<O, 256, 256, 2, 4, 1>(g, 4, st);
-  if (mid < small) return go_tiles<O, 128, 128, 4, 2, 2>(g, 8, st);
+  if (mid < small) {
+    if constexpr (std::is_same_v<O, F32>) return go_tiles<O, 128, 128, 2, 2, 2>(g, 8, st);  // (its registers do not fit eight waves)
+    else return go_tiles<O, 128, 128, 4, 2, 2>(g, 8, st);
+  }
   return go_tiles<O, 64, 64, 2, 2, 4>(g, 8, st);
 }
 

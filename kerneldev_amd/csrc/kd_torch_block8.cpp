@@ -7,6 +7,8 @@
 // kernels run for 40 us, takes 100 us through the Python nodes.
 #include <torch/library.h>
 
+#include <ATen/hip/EmptyTensor.h>
+
 #include "kd_torch.h"
 
 namespace {
@@ -37,13 +39,18 @@ Tensor rows_ready(const Tensor& t) {  // [rows, cols], rows a multiple of 8 elem
   return t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && aligned16(t) ? t : flat(t);
 }
 
+// New memory on t's device (not through the dispatcher, which takes longer than the allocator)
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& t) {
+  return Tensor(at::detail::empty_cuda(sizes, type, t.device(), std::nullopt));
+}
+
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 Tensor bytes8(const Tensor& like, int64_t rows, int64_t cols) {
-  return at::empty({rows, up16(cols)}, like.options().dtype(at::kFloat8_e4m3fn));
+  return fresh({rows, up16(cols)}, at::kFloat8_e4m3fn, like);
 }
 Tensor scales(const Tensor& like, int64_t rows, int64_t nb) {
-  return at::empty({rows, nb}, like.options().dtype(at::kFloat8_e8m0fnu));
+  return fresh({rows, nb}, at::kFloat8_e8m0fnu, like);
 }
 uint8_t* u8(const Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
@@ -126,7 +133,7 @@ Tensor matmul8(const Tensor& a_in, const Tensor& a_scale, const Tensor& b_in, co
   TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31), "M, N and K must be < 2^31");
   kd_matmul8_args g{};
   g.dtype = dtype_code(out_type, true), g.fast = fast;
-  Tensor out = at::empty({M, N}, a.options().dtype(out_type));
+  Tensor out = fresh({M, N}, out_type, a);
   if (out.numel() == 0) return out;
   g.a = u8(a), g.b = u8(b), g.lda = a.stride(0), g.ldb = b.stride(0), g.a_scale = u8(as), g.b_scale = u8(bs);
   g.out = out.data_ptr(), g.ldo = N;
@@ -140,7 +147,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm8(const Tensor& x_in, const OptTe
   TORCH_CHECK_VALUE(x_in.dim() == 2, "x must be a matrix");
   const c10::DeviceGuard on(x_in.device());
   const Tensor x = flat(x_in);
-  Tensor d, sum = at::empty({0}, x.options());
+  Tensor d, sum;
   kd_norm8_args a{};
   a.dtype = dtype_code(x.scalar_type(), false);
   a.rows = x.size(0), a.D = int32_t(x.size(1)), a.eps = float(eps);
@@ -148,10 +155,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm8(const Tensor& x_in, const OptTe
     on_one_gpu({&x, &*delta});
     TORCH_CHECK_VALUE(delta->sizes() == x.sizes() && delta->scalar_type() == x.scalar_type(),
                       "x and delta must have one shape and type");
-    d = flat(*delta), sum = at::empty(x.sizes(), x.options());
+    d = flat(*delta), sum = fresh(x.sizes(), x.scalar_type(), x);
     a.delta = d.data_ptr(), a.sum = sum.data_ptr();
   }
-  Tensor y = bytes8(x, a.rows, a.D), s = scales(x, a.rows, blocks(a.D)), rstd = at::empty({a.rows}, x.options().dtype(at::kFloat));
+  Tensor y = bytes8(x, a.rows, a.D), s = scales(x, a.rows, blocks(a.D)), rstd = fresh({a.rows}, at::kFloat, x);
+  if (!delta) sum = fresh({0}, x.scalar_type(), x);
   if (a.rows == 0) return {sum, y, s, rstd};
   a.x = x.data_ptr(), a.y = u8(y), a.y_stride = y.stride(0), a.scale = u8(s), a.rstd = static_cast<float*>(rstd.data_ptr());
   check(kd_norm8(&a, stream_of(x)), "kd_norm8");
@@ -175,7 +183,7 @@ Tensor norm8_bwd(const Tensor& g_in, const OptTensor& ds, const Tensor& y, const
   }
   kd_norm8_bwd_args a{};
   a.dtype = dtype_code(dtype, false), a.g_dtype = dtype_code(g.scalar_type(), true);
-  Tensor dx = at::empty(g.sizes(), g.options().dtype(dtype));
+  Tensor dx = fresh(g.sizes(), dtype, g);
   a.rows = g.size(0), a.D = int32_t(g.size(1));
   if (a.rows == 0) return dx;
   a.g = g.data_ptr(), a.ds = ds ? d.data_ptr() : nullptr, a.y = u8(y), a.y_stride = y.stride(0), a.scale = u8(scale);
@@ -211,7 +219,7 @@ std::tuple<Tensor, Tensor> gate8_bwd(const Tensor& dy_in, const Tensor& a8, cons
   check_blocks(a8, as, dy_in.size(1), 1, "a"), check_blocks(b8, bs, dy_in.size(1), 1, "b");
   const c10::DeviceGuard on(dy_in.device());
   const Tensor dy = flat(dy_in);
-  Tensor da = at::empty(dy.sizes(), dy.options().dtype(dtype)), db = at::empty(dy.sizes(), dy.options().dtype(dtype));
+  Tensor da = fresh(dy.sizes(), dtype, dy), db = fresh(dy.sizes(), dtype, dy);
   kd_gate8_args g{};
   g.dtype = dtype_code(dtype, false), g.dy_dtype = dtype_code(dy.scalar_type(), true);
   g.rows = dy.size(0), g.H = int32_t(dy.size(1));
@@ -245,11 +253,11 @@ Tensor weight_grad8(at::TensorList dys, const Tensor& x, const Tensor& x_scale, 
   TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31), "M and N must be < 2^31");
   g.dtype = dtype_code(dys[0].scalar_type(), false);
   if (M == 0) return at::zeros({N, K}, dys[0].options());
-  Tensor dw = at::empty({N, K}, dys[0].options());
+  Tensor dw = fresh({N, K}, dys[0].scalar_type(), x);
   g.M = int32_t(M), g.N = int32_t(N), g.K = int32_t(K);
   g.ws_bytes = kd_weight_grad8_ws_bytes(g.M, g.N, g.K, g.dtype);
   check(g.ws_bytes < 0 ? KD_ERR_UNSUPPORTED : KD_OK, "kd_weight_grad8");
-  const Tensor ws = at::empty({g.ws_bytes}, dys[0].options().dtype(at::kByte));
+  const Tensor ws = fresh({g.ws_bytes}, at::kByte, x);
   g.x = u8(x), g.ldx = x.stride(0), g.x_scale = u8(x_scale);
   g.dw = dw.data_ptr(), g.ws = static_cast<float*>(ws.data_ptr());
   check(kd_weight_grad8(&g, stream_of(x)), "kd_weight_grad8");
@@ -272,7 +280,7 @@ Tensor embed(const Tensor& tokens_in, const Tensor& weight_in, double scale) {
   const Tensor tokens = tokens_in.contiguous(), weight = weight_in.contiguous();
   auto shape = tokens_in.sizes().vec();
   shape.push_back(weight.size(1));
-  Tensor out = at::empty(shape, weight.options());
+  Tensor out = fresh(shape, weight.scalar_type(), weight);
   kd_embed_args a = embed_args(tokens, weight.size(0), weight.size(1), weight.scalar_type(), scale);
   if (out.numel() == 0) return out;
   a.weight = weight.data_ptr(), a.out = out.data_ptr();
@@ -288,9 +296,9 @@ Tensor embed_grad(const Tensor& tokens_in, const Tensor& dy_in, int64_t vocab, d
   TORCH_CHECK_VALUE(dy.dim() >= 1 && tokens.numel() * dim == dy.numel(), "dy must be tokens' shape by dim");
   kd_embed_args a = embed_args(tokens, vocab, dim, dy.scalar_type(), scale);
   if (dy.numel() == 0) return at::zeros({vocab, dim}, dy.options());
-  Tensor dw = at::empty({vocab, dim}, dy.options());
+  Tensor dw = fresh({vocab, dim}, dy.scalar_type(), dy);
   const int64_t need = kd_embed_grad_ws_bytes(a.n, vocab, dim);
-  const Tensor ws = at::empty({std::max<int64_t>(need, 0)}, dy.options().dtype(at::kByte));
+  const Tensor ws = fresh({std::max<int64_t>(need, 0)}, at::kByte, dy);
   a.dy = dy.data_ptr(), a.dw = dw.data_ptr(), a.padding_idx = padding_idx;
   check(kd_embed_grad(&a, ws.data_ptr(), need, stream_of(dy)), "kd_embed_grad");
   return dw;

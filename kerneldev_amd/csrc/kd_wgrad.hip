@@ -152,12 +152,14 @@ struct Wgrad8Args {
   int M, N, K, S, tn, tk, nb;
 };
 
-// 16 e4m3 bytes times the scale as 16 bf16
-KD_DEV void widen16(const u32x4& v, float scale, u32x4 (&out)[2]) {
+// 8 e4m3 bytes times the scale as 8 bf16
+KD_DEV u32x4 widen8(const u32x2& v, float scale) {
+  u32x4 w;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    out[i >> 2][i & 3] = __builtin_bit_cast(uint32_t, (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i >> 1], scale, true)
-                                                              : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i >> 1], scale, false));
+  for (int i = 0; i < 4; ++i)
+    w[i] = __builtin_bit_cast(uint32_t, (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i >> 1], scale, true)
+                                                : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i >> 1], scale, false));
+  return w;
 }
 
 template <class E>
@@ -187,27 +189,31 @@ __global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args w) {
     const u32x4 rs = rsrc_words(dy + int64_t(e) * 64 * yrb, rows > 0 ? uint32_t(rows - 1) * yrb + uint32_t(cols) * 2u : 0u);
     TL::load_async(rs, uint32_t(first) * 2u, yoff, lds_addr(s_y[slot]), wave);
   };
-  const int xr = tid >> 2, xc = k0 + (tid & 3) * 32;  // this thread's row of a step and its first column
-  const uint32_t xo[2] = {xc < w.K ? uint32_t(xr * w.ldx) + xc : OFF_OUTSIDE, xc + 16 < w.K ? uint32_t(xr * w.ldx) + xc + 16 : OFF_OUTSIDE};
-  u32x4 xv[2];
+  // This thread's row of a step and its 32 columns, in four words whose order turns
+  // with the thread: the 16 lanes that write at once then meet every bank once
+  const int xr = tid >> 2;
+  uint32_t xo[4];
+  int xto[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int ch = 4 * (tid & 3) + ((q + tid) & 3), col = k0 + 8 * ch;
+    xo[q] = col < w.K ? uint32_t(xr * w.ldx) + uint32_t(col) : OFF_OUTSIDE;
+    xto[q] = TL::at(xr, ch);
+  }
+  u32x2 xv[4];
   uint32_t xs;
   auto load_x = [&](int e) {  // (rows and columns outside: zeros)
     const int rows = max(0, min(64, w.M - e * 64));
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(w.x + int64_t(e) * 64 * w.ldx, rows > 0 ? uint32_t((rows - 1) * w.ldx + (w.K + 15) / 16 * 16) : 0u),
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(w.x + int64_t(e) * 64 * w.ldx, rows > 0 ? uint32_t((rows - 1) * w.ldx + w.K) : 0u),
                                  rsc = make_rsrc(w.scale + int64_t(e) * 64 * w.nb, uint32_t(rows * w.nb));
 #pragma unroll
-    for (int q = 0; q < 2; ++q) xv[q] = buf_load16(r, xo[q]);
+    for (int q = 0; q < 4; ++q) xv[q] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, xo[q], 0, 0));
     xs = __builtin_amdgcn_raw_buffer_load_b8(rsc, uint32_t(xr * w.nb + kb), 0, 0);
   };
   auto put_x = [&](int slot) {
     const float s = scale_value(xs);
-    u32x4 o[2];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      widen16(xv[q], s, o);
-      *reinterpret_cast<u32x4*>(s_x[slot] + TL::at(xr, 4 * (tid & 3) + 2 * q)) = o[0];
-      *reinterpret_cast<u32x4*>(s_x[slot] + TL::at(xr, 4 * (tid & 3) + 2 * q + 1)) = o[1];
-    }
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<u32x4*>(s_x[slot] + xto[q]) = widen8(xv[q], s);
   };
   const int wn = wave >> 1, wk = wave & 1;
   int ya[2][2], xa[2][2];
@@ -230,13 +236,13 @@ __global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args w) {
   load_x(e0);
   load_y(e0, 0);
   wait_vmem();
-  settle(xv[0]), settle(xv[1]), settle(xs);
+  settle(xv[0]), settle(xv[1]), settle(xv[2]), settle(xv[3]), settle(xs);
   put_x(0);
   load_x(e0 + 1);
   for (int e = e0; e < e1; ++e) {  // (one basic block: copies of a step behind the piece are read by nobody)
     const int slot = (e - e0) & 1;
     wait_vmem();
-    settle(xv[0]), settle(xv[1]), settle(xs);
+    settle(xv[0]), settle(xv[1]), settle(xv[2]), settle(xv[3]), settle(xs);
     barrier_lds();  // the step's tiles are in place for every wave, and every wave is done with the other slot
     load_y(e + 1, slot ^ 1);
     lds_u8 *ty = to_lds(s_y[slot]), *tx = to_lds(s_x[slot]);
@@ -256,8 +262,8 @@ __global__ __launch_bounds__(256, 2) void k_wgrad8(Wgrad8Args w) {
         for (int b = 0; b < 2; ++b)
           av[(ks + 1) & 1][b] = read(ty, ya[b], ks + 1), bv[(ks + 1) & 1][b] = read(tx, xa[b], ks + 1);
       }
-      if (ks == 1) put_x(slot ^ 1);
-      if (ks == 2) load_x(e + 2);
+      if (ks == 0) put_x(slot ^ 1);
+      if (ks == 1) load_x(e + 2);
       __builtin_amdgcn_sched_barrier(0x406);
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
