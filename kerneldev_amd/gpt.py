@@ -20,6 +20,12 @@ double loop, and the scores are fp32.
 
 ``attention`` is injectable so a test can run the same weights through a
 dense fp32 reference attention.
+
+``projections="fp8_e4m3"`` runs the blocks' projections on 8-bit blocks
+(``block_fp8.py``): each norm takes in the residual's addition and feeds q, k and v
+or the gate in one product, the activations kept for the backward are 8-bit, and
+the token embedding's gradient is summed by sorted tokens (``embed.py``).  The
+parameters, and the default, are the same.
 """
 from __future__ import annotations
 
@@ -29,6 +35,8 @@ import torch.nn.functional as F
 
 from . import _lib
 from .attention import AttentionPlan, build_plan, build_plan_from_tokens, flash_attention, mask_mode
+from .block_fp8 import fp8_projection, norm_projection, swiglu_projection
+from .embed import embedding
 from .metadata import CLS, MASKQ, SPAN, derive_metadata
 from .span_head import has_cocktail_layout, span_scores
 
@@ -99,11 +107,14 @@ class MultiHeadAttention(nn.Module):
         self.attention = attention or flash_attention
 
     def forward(self, x, in_span, span_id, is_prefix, plan=None):
-        B, L, _ = x.shape
+        out = self.attend(self.q_proj(x), self.k_proj(x), self.v_proj(x), in_span, span_id, is_prefix, plan)
+        return self.o_proj(out)
+
+    def attend(self, q, k, v, in_span, span_id, is_prefix, plan=None):
+        """Attention of projected rows [B, L, H d], as rows."""
+        B, L, _ = q.shape
         shape = (B, L, self.n_heads, self.head_dim)
-        q = self.q_proj(x).view(shape).transpose(1, 2)
-        k = self.k_proj(x).view(shape).transpose(1, 2)
-        v = self.v_proj(x).view(shape).transpose(1, 2)
+        q, k, v = (t.view(shape).transpose(1, 2) for t in (q, k, v))
         if plan is not None:  # the model's shared plan stands for the metadata
             # flash_attention writes O straight into [B, L, H, d] memory, so the
             # transpose + reshape below is a view rather than model.py:95's copy
@@ -111,7 +122,7 @@ class MultiHeadAttention(nn.Module):
         else:
             out = self.attention(q, k, v, lens=None, causal=self.causal, attention_mask=None,
                                  in_span=in_span, span_id=span_id, is_prefix=is_prefix)
-        return self.o_proj(out.transpose(1, 2).reshape(B, L, -1))
+        return out.transpose(1, 2).reshape(B, L, -1)
 
 
 class Block(nn.Module):
@@ -125,13 +136,25 @@ class Block(nn.Module):
         x = x + self.attn(self.norm1(x), in_span, span_id, is_prefix, plan)
         return x + self.mlp(self.norm2(x))
 
+    def forward_fp8(self, x, delta, in_span, span_id, is_prefix, plan=None):
+        """The block on 8-bit projections.  The rows are x + delta, delta the last layer's output (None: none yet);
+        returned are the rows before the block's last addition and what is to be added."""
+        attn, mlp = self.attn, self.mlp
+        x, q, k, v = norm_projection(x, delta, attn.q_proj.weight, attn.k_proj.weight, attn.v_proj.weight, eps=self.norm1.eps)
+        out = fp8_projection(attn.attend(q, k, v, in_span, span_id, is_prefix, plan), attn.o_proj.weight)
+        x, a, b = norm_projection(x, out, mlp.w1.weight, mlp.w3.weight, eps=self.norm2.eps)
+        return x, swiglu_projection(a, b, mlp.w2.weight)
+
 
 class GPTModel(nn.Module):
     """Config 5: d_model 768, 12 layers, 12 heads of 64, SwiGLU 2048, vocab 262."""
 
     def __init__(self, vocab_size=VOCAB, dim=768, n_layers=12, n_heads=12, max_seq_len=2048, mlp_hidden=2048,
-                 causal=True, attention=None):
+                 causal=True, attention=None, projections=None):
         super().__init__()
+        if projections not in (None, "fp8_e4m3"):
+            raise ValueError(f"projections must be None or 'fp8_e4m3', got {projections!r}")
+        self.projections = projections
         self.token_emb = nn.Embedding(vocab_size, dim)
         self.pos_emb = nn.Embedding(max_seq_len, dim)
         self.blocks = nn.ModuleList(Block(dim, n_heads, mlp_hidden, causal, attention) for _ in range(n_layers))
@@ -144,6 +167,11 @@ class GPTModel(nn.Module):
 
     def hidden(self, tokens, in_span, span_id, is_prefix, plan=None):
         pos = torch.arange(tokens.shape[1], device=tokens.device)
+        if self.projections is not None:
+            h, delta = embedding(tokens, self.token_emb.weight) + self.pos_emb(pos)[None], None
+            for blk in self.blocks:
+                h, delta = blk.forward_fp8(h, delta, in_span, span_id, is_prefix, plan)
+            return self.norm_out(h if delta is None else h + delta)
         h = self.token_emb(tokens) + self.pos_emb(pos)[None]
         for blk in self.blocks:
             h = blk(h, in_span, span_id, is_prefix, plan)

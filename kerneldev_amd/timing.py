@@ -68,7 +68,8 @@ def time_gpt_step(attention="kdattn", B=8, L=2048, steps=5, warmup=2, seed=4):
     batch, span-score cross entropy, backward and an AdamW update (the step of
     train_loop.py's inner loop, without its DDP and logging).
 
-    ``attention``: ``"kdattn"`` (flash_attention, one plan shared by the layers),
+    ``attention``: ``"kdattn"`` (flash_attention, one plan shared by the layers), ``"kdattn_fp8"`` (the same with the
+    projections on 8-bit blocks),
     ``"sdpa_bf16"`` (torch SDPA in bf16 on its memory-efficient backend with the
     dense mask) or ``"sdpa_fp32"`` (torch SDPA in fp32, math backend).  The
     dense mask comes from flash_attention's own mask output and is built once,
@@ -80,8 +81,8 @@ def time_gpt_step(attention="kdattn", B=8, L=2048, steps=5, warmup=2, seed=4):
     dev = torch.device("cuda:0")
     tokens, in_span, span_id, is_prefix, correct = (x.to(dev) for x in config5_batch(B=B, L=L, seed=seed))
     torch.manual_seed(seed)
-    if attention == "kdattn":
-        model = GPTModel(max_seq_len=L)
+    if attention in ("kdattn", "kdattn_fp8"):
+        model = GPTModel(max_seq_len=L, projections="fp8_e4m3" if attention == "kdattn_fp8" else None)
     else:
         probe = torch.zeros(B, 1, L, 64, device=dev, dtype=torch.bfloat16)
         _, mask = flash_attention(probe, probe, probe, return_attention_mask=True,
@@ -111,7 +112,7 @@ def time_gpt_step(attention="kdattn", B=8, L=2048, steps=5, warmup=2, seed=4):
 
 def main():
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("--gpt", nargs="*", choices=("kdattn", "sdpa_bf16", "sdpa_fp32"),
+    ap.add_argument("--gpt", nargs="*", choices=("kdattn", "kdattn_fp8", "sdpa_bf16", "sdpa_fp32"),
                     help="time config-5 training steps with these attentions instead")
     ap.add_argument("--dtype", default="bf16", choices=tuple(DTYPES))
     ap.add_argument("--precision", default="tf32", choices=("tf32", "ieee", "bf16"))
