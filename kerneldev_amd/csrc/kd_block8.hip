@@ -115,13 +115,13 @@ KD_DEV void turn4(const uint32_t (&r)[4], uint32_t (&c)[4]) {
   c[2] = __builtin_amdgcn_perm(t3, t2, 0x05040100u), c[3] = __builtin_amdgcn_perm(t3, t2, 0x07060302u);
 }
 
-// A workgroup a block of 128 x 128, a thread 8 rows of 8 columns: the bytes go out
+// A workgroup a block of 128 x 128, a thread 4 rows of 8 columns: the bytes go out
 // as they are and, turned over in registers, transposed.  Latency bounds it (a
 // model's weight is some hundred blocks): one round of loads, one exchange of the
-// maximum (16384 tokens' q, k and v, 2304 x 768: 4 us; through LDS, byte by byte, 10).
+// maximum.
 template <class E>
-__global__ __launch_bounds__(256) void k_quant_weight(kd_weight8_args a, uint32_t kblocks, uint32_t nblocks) {
-  __shared__ uint32_t s_max[4];
+__global__ __launch_bounds__(512) void k_quant_weight(kd_weight8_args a, uint32_t kblocks, uint32_t nblocks) {
+  __shared__ uint32_t s_max[8];
   const int tid = threadIdx.x, nb = blockIdx.x / kblocks, kb = blockIdx.x - nb * kblocks;
   const void* src = a.w[0];  // the part that holds this block (parts before the last: whole blocks)
   int64_t stride = a.w_stride[0];
@@ -129,45 +129,55 @@ __global__ __launch_bounds__(256) void k_quant_weight(kd_weight8_args a, uint32_
 #pragma unroll
   for (int i = 1; i < 4; ++i)
     if (i < a.n && first >= height) first -= height, src = a.w[i], stride = a.w_stride[i], height = a.rows[i];
-  const int rows = min(QB, height - first), r0 = (tid >> 4) * 8, col = kb * QB + (tid & 15) * 8;
-  float f[8][8];
+  const int rows = min(QB, height - first), r0 = (tid >> 4) * 4, col = kb * QB + (tid & 15) * 8;
+  float f[4][8];
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     zero8(f[i]);
     if (r0 + i < rows && col < a.K) load8<E>(src, int64_t(first + r0 + i) * stride + col, f[i]);
   }
+  auto block_max = [&](uint32_t v) {
+    v = row16_max(v);
+    v = max(v, uint32_t(__shfl_xor(int(v), 16, 64)));
+    v = max(v, uint32_t(__shfl_xor(int(v), 32, 64)));
+    if ((tid & 63) == 0) s_max[tid >> 6] = v;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, finite_max(f[i]));
-  m = row16_max(m);
-  m = max(m, uint32_t(__shfl_xor(int(m), 16, 64)));
-  m = max(m, uint32_t(__shfl_xor(int(m), 32, 64)));
-  if ((tid & 63) == 0) s_max[tid >> 6] = m;
-  __syncthreads();
-  m = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+    for (int i = 0; i < 8; ++i) v = max(v, s_max[i]);
+    return v;
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, any_max(f[i]));
+  m = block_max(m);
+  const bool finite = m < 0x7F800000u;  // (the same in every thread; blocks that hold a NaN or an infinity take the longer way)
+  if (!finite) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, finite_max(f[i]));
+    __syncthreads();  // (the maxima above are read)
+    m = block_max(m);
+  }
   const uint32_t b = scale_byte(m);
-  const float inv = scale_inverse(b);
   if (tid == 0) {
     a.scale[int64_t(nb) * kblocks + kb] = uint8_t(b);
     if (a.scale_t != nullptr) a.scale_t[int64_t(kb) * nblocks + nb] = uint8_t(b);
   }
-  u32x2 w[8];
+  u32x2 w[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = pack_e4m3(f[i], inv);
+  for (int i = 0; i < 4; ++i) {
+    w[i] = finite ? pack_finite(f[i], scale_value(b)) : pack_e4m3(f[i], scale_inverse(b));
     if (r0 + i < rows && col < (a.K + 15) / 16 * 16)
       *reinterpret_cast<u32x2*>(a.y + (int64_t(nb) * QB + r0 + i) * a.y_stride + col) = w[i];
   }
   if (a.yt == nullptr || nb * QB + r0 >= (a.total + 15) / 16 * 16) return;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t lo[4], hi[4];
-    turn4({w[0][h], w[1][h], w[2][h], w[3][h]}, lo);
-    turn4({w[4][h], w[5][h], w[6][h], w[7][h]}, hi);
+    uint32_t t[4];
+    turn4({w[0][h], w[1][h], w[2][h], w[3][h]}, t);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (col + 4 * h + j < a.K)
-        *reinterpret_cast<u32x2*>(a.yt + int64_t(col + 4 * h + j) * a.yt_stride + nb * QB + r0) = u32x2{lo[j], hi[j]};
+      if (col + 4 * h + j < a.K) *reinterpret_cast<uint32_t*>(a.yt + int64_t(col + 4 * h + j) * a.yt_stride + nb * QB + r0) = t[j];
   }
 }
 
@@ -374,7 +384,7 @@ int launch_quant_rows(const kd_rows8_args& a, hipStream_t st) {
 int launch_quant_weight(const kd_weight8_args& a, hipStream_t st) {
   const uint32_t kb = uint32_t((a.K + QB - 1) / QB), nb = uint32_t((a.total + QB - 1) / QB);
   auto go = [&](auto e) {
-    hipLaunchKernelGGL(k_quant_weight<decltype(e)>, dim3(kb * nb), dim3(256), 0, st, a, kb, nb);
+    hipLaunchKernelGGL(k_quant_weight<decltype(e)>, dim3(kb * nb), dim3(512), 0, st, a, kb, nb);
   };
   if (a.dtype == KD_F32) {
     go(F32{});

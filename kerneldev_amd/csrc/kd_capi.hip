@@ -377,6 +377,7 @@ static int check_wgrad8(int32_t M, int32_t N, int32_t K, int32_t dtype) {
   if (N % 8 != 0 || K % 8 != 0) return fail(KD_ERR_UNSUPPORTED, "N and K must be multiples of 8");
   if (N > (1 << 22) || K > (1 << 22) || int64_t(N) * K >= (int64_t(1) << 30))
     return fail(KD_ERR_UNSUPPORTED, "N and K must be <= 2^22 and dW < 2^30 elements");
+  if (M > 0x7FFFFF00) return fail(KD_ERR_UNSUPPORTED, "M must be <= 2^31 - 256");
   if (!type16(dtype)) return fail(KD_ERR_UNSUPPORTED, "dtype must be bf16 or fp16");
   return KD_OK;
 }
