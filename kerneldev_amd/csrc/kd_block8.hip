@@ -80,30 +80,46 @@ KD_DEV void store_block(const u32x4& v, uint8_t* y, int64_t y_stride, uint8_t* s
   store_bytes(w, b, y, y_stride, scale, nb, row, col, cols);
 }
 
-template <class E>
+// U blocks a DPP row of lanes, 16 apart: their loads go out together
+template <class E, int U>
 __global__ __launch_bounds__(256) void k_quant_rows(kd_rows8_args a, int64_t row0, uint32_t blocks, uint32_t nb) {
-  const uint32_t blk = blockIdx.x * 16u + (threadIdx.x >> 4);
-  const uint32_t r = blk / nb, kb = blk - r * nb;
-  const int64_t row = row0 + r;
-  const int col = int(kb) * QB + int(threadIdx.x & 15) * 8;
-  if (blk >= blocks) return;  // (whole DPP rows)
-  // the part that holds the column (parts before the last end on a block's edge)
-  const void* x = a.x[0];
-  int64_t stride = a.x_stride[0];
-  int c = col, cols = a.cols[0];
+  u32x4 v[U], hi[U];
+  int64_t row[U];
+  int col[U];
+  const uint32_t blk0 = blockIdx.x * (16u * U) + (threadIdx.x >> 4);
 #pragma unroll
-  for (int i = 1; i < 4; ++i)
-    if (i < a.n && c >= cols) c -= cols, x = a.x[i], stride = a.x_stride[i], cols = a.cols[i];
-  const int64_t at = row * stride + c;
-  if constexpr (std::is_same_v<E, F32>) {
-    float f[8];
-    zero8(f);
-    if (col < a.total) load8<F32>(x, at, f);
-    store_block(f, a.y, a.y_stride, a.scale, nb, row, col, a.total);
-  } else {
-    u32x4 v{};
-    if (col < a.total) v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + at);
-    store_block<E>(v, a.y, a.y_stride, a.scale, nb, row, col, a.total);
+  for (int u = 0; u < U; ++u) {
+    const uint32_t blk = min(blk0 + 16u * u, blocks - 1), r = blk / nb, kb = blk - r * nb;  // (behind the last: the last)
+    row[u] = row0 + r, col[u] = int(kb) * QB + int(threadIdx.x & 15) * 8;
+    // the part that holds the column (parts before the last end on a block's edge)
+    const void* x = a.x[0];
+    int64_t stride = a.x_stride[0];
+    int c = col[u], cols = a.cols[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if (i < a.n && c >= cols) c -= cols, x = a.x[i], stride = a.x_stride[i], cols = a.cols[i];
+    const int64_t at = row[u] * stride + c;
+    v[u] = hi[u] = u32x4{};
+    if (col[u] < a.total) {
+      if constexpr (std::is_same_v<E, F32>) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(x) + at);
+        v[u] = p[0], hi[u] = p[1];
+      } else {
+        v[u] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + at);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (blk0 + 16u * u >= blocks) return;  // (whole DPP rows)
+    if constexpr (std::is_same_v<E, F32>) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(v[u][i]), f[4 + i] = __uint_as_float(hi[u][i]);
+      store_block(f, a.y, a.y_stride, a.scale, nb, row[u], col[u], a.total);
+    } else {
+      store_block<E>(v[u], a.y, a.y_stride, a.scale, nb, row[u], col[u], a.total);
+    }
   }
 }
 
@@ -366,19 +382,24 @@ void norm_variant(int D, G go) {  // waves a row and words a lane
 
 }  // namespace
 
+// Two blocks a thread where there are many, 16 bits (us, one and two): 16384 x 2304 26.9 and 24.2, 16384 x 768 8.8 and
+// 8.3, but 2048 x 768 2.6 and 2.9, 633 x 1000 2.3 and 2.7; four 27.3, 9.1, 3.9, 3.9.  fp32: 16384 x 768 11.4 and 11.7.
 int launch_quant_rows(const kd_rows8_args& a, hipStream_t st) {
   const uint32_t nb = uint32_t((a.total + QB - 1) / QB);
-  auto go = [&](auto e) {
+  auto go = [&](auto e, auto u) {
+    constexpr int U = decltype(u)::value;
     in_launches(a.rows, 16 * int64_t(nb), [&](int64_t r, int64_t n) {
       const uint32_t blocks = uint32_t(n) * nb;
-      hipLaunchKernelGGL(k_quant_rows<decltype(e)>, dim3((blocks + 15) / 16), dim3(256), 0, st, a, r, blocks, nb);
+      hipLaunchKernelGGL((k_quant_rows<decltype(e), U>), dim3((blocks + 16 * U - 1) / (16 * U)), dim3(256), 0, st, a, r, blocks, nb);
     });
   };
+  using one = std::integral_constant<int, 1>;
+  using two = std::integral_constant<int, 2>;
   if (a.dtype == KD_F32) {
-    go(F32{});
+    go(F32{}, one{});
     return hipGetLastError() == hipSuccess ? KD_OK : KD_ERR_LAUNCH;
   }
-  return by_type(a.dtype, go);
+  return by_type(a.dtype, [&](auto e) { a.rows * nb >= (1 << 16) ? go(e, two{}) : go(e, one{}); });
 }
 
 int launch_quant_weight(const kd_weight8_args& a, hipStream_t st) {
