@@ -50,7 +50,15 @@ KD_DEV void tile_of(int item, int tiles_m, int tiles_n, int group, int* tm, int*
 // read while the products of the part before run; before the last part, when every
 // wave has read all of the step's, the next step's tiles must have landed and the
 // copies of the step behind it start: about a step's products to arrive in, and one
-// barrier a step.  C leaves through LDS in whole rows.
+// barrier a step.  Reads and copies stand between single products (all ahead of a
+// part's products: 5 % slower).  C leaves through LDS in whole rows.
+//
+// What bounds it: in 8192^3, 450 us or 2.4 PFLOP/s, the products are issued half of the
+// time; the waves' reads keep the LDS three quarters busy and the copies' writes the
+// rest.  Four waves of 128 x 128, which read two thirds of that, have nobody to take
+// over while they wait: 487 us.  Workgroups that go on to a next tile, with its copies
+// on their way while C is stored from registers: 489, and 50 against 47 in 16384 x
+// 2304 x 768.
 template <class O, int BM, int BN, int WM, int WN, int PER_CU>
 struct Gemm8 {
   static constexpr bool F = std::is_same_v<O, F32>, WIDE = F || std::is_same_v<O, F32Q>;
@@ -90,13 +98,13 @@ __global__ __launch_bounds__(64 * WM * WN, (PER_CU * WM * WN + 3) / 4) void k_ge
                         : rsrc_words(g.b + int64_t(n0) * g.ldb, uint32_t(int64_t(rows_b - 1) * g.ldb + g.K));
   const uint32_t arow = uint32_t(piece0 * 8 + lane / TL::CPR) * ld,
                  c16 = uint32_t((lane % TL::CPR) ^ TL::swz(lane / TL::CPR)) * 16u;
-  auto load = [&](int e) {  // (of a step behind the last: zeros)
+  auto load = [&](int e, int from, int to) {  // copies from .. to - 1 of step e (of a step behind the last: zeros)
     const uint32_t k0 = uint32_t(e) * QB;
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(s_pool) + uint32_t(e & 1) * G::SLOT + uint32_t(wave * LOADS) * 1024u);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(lds_addr(s_pool) + uint32_t(e & 1) * G::SLOT + uint32_t(wave * LOADS) * 1024u);
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
+    for (int j = from; j < to; ++j) {
       const uint32_t col = k0 + (c16 ^ ((j & 1) * uint32_t(TL::swz(8)) * 16u));
-      dma_b128(rs, col < uint32_t(g.K) ? arow + uint32_t(j * 8) * ld + col : OFF_OUTSIDE, to + uint32_t(j) * 1024u);
+      dma_b128(rs, col < uint32_t(g.K) ? arow + uint32_t(j * 8) * ld + col : OFF_OUTSIDE, at + uint32_t(j) * 1024u);
     }
   };
   // Scales, SB blocks of K at a time, in two buffers: a thread takes SPT bytes of a
@@ -119,7 +127,7 @@ __global__ __launch_bounds__(64 * WM * WN, (PER_CU * WM * WN + 3) / 4) void k_ge
     if (tid < G::NBT * G::SB) to[(BM + tid / G::SB) * G::SROW + tid % G::SB] = uint8_t(sw);
   };
   fetch_scales(0);
-  load(0);
+  load(0, 0, LOADS);
   put_scales(0);
   const int wn = wave / WM, wm = wave - wn * WM;
   f32x16 acc[FB][FA];  // [32 rows of B][32 rows of A]
@@ -134,30 +142,25 @@ __global__ __launch_bounds__(64 * WM * WN, (PER_CU * WM * WN + 3) / 4) void k_ge
     return join8(ds_read16(t + (at0 ^ (64 * h))), ds_read16(t + (at1 ^ (64 * h))));
   };
   uint32_t xs[FA], ws = 0;  // scale bytes, the current block's lowest
-  auto multiply = [&](const i32x8& a, const i32x8 (&b)[FB], int j) {
+  auto multiply = [&](const i32x8& a, const i32x8& b, int i, int j) {
+    if constexpr (F) {
+      f32x16 part{};  // without the scales
 #pragma unroll
-    for (int i = 0; i < FB; ++i) {
-      if constexpr (F) {
-        f32x16 part{};  // without the scales
+      for (int q = 0; q < 4; ++q) part = mfma32x32x16<BF16>(as_bf16(b, q), as_bf16(a, q), part);
+      const int e2 = int(ws & 255u) + int(xs[j] & 255u) - 254;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) part = mfma32x32x16<BF16>(as_bf16(b[i], q), as_bf16(a, q), part);
-        const int e2 = int(ws & 255u) + int(xs[j] & 255u) - 254;
-#pragma unroll
-        for (int q = 0; q < 16; ++q) acc[i][j][q] += __builtin_amdgcn_ldexpf(part[q], e2);
-      } else {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[i], a, acc[i][j], 0, 0, 0, int(ws), 0, int(xs[j]));
-      }
+      for (int q = 0; q < 16; ++q) acc[i][j][q] += __builtin_amdgcn_ldexpf(part[q], e2);
+    } else {
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, acc[i][j], 0, 0, 0, int(ws), 0, int(xs[j]));
     }
   };
   i32x8 fa[2], fb[2][FB];  // A's 32 rows of this part and the next; B's of this half and the next
-  auto read_b = [&](int e, int h) {
-#pragma unroll
-    for (int i = 0; i < FB; ++i) fb[h][i] = frag(e, h, BM + wn * G::TN + 32 * i);
-  };
+  auto read_b = [&](int e, int h, int i) { fb[h][i] = frag(e, h, BM + wn * G::TN + 32 * i); };
   wait_vmem();
   barrier_lds();  // the first step's tiles and scales are in place for every wave
-  load(1);        // (copies of steps behind the last write zeros)
-  read_b(0, 0);
+  load(1, 0, LOADS);  // (copies of steps behind the last write zeros)
+#pragma unroll
+  for (int i = 0; i < FB; ++i) read_b(0, 0, i);
   fa[0] = frag(0, 0, wm * G::TM);
   for (int e0 = 0; e0 < nb; e0 += G::SB) {
     const int chunk = e0 / G::SB, e1 = min(nb, e0 + G::SB);
@@ -176,20 +179,25 @@ __global__ __launch_bounds__(64 * WM * WN, (PER_CU * WM * WN + 3) / 4) void k_ge
     // One basic block: products would otherwise sink past the barrier, behind the reads they are to cover
     for (int e = e0; e < e1; ++e) {
 #pragma unroll
-      for (int t = 0; t < 2 * FA; ++t) {  // part t: half t / FA, A's rows 32 (t % FA) on
-        if (t == 2 * FA - 1) {
-          wait_vmem();
-          barrier_lds();  // step e + 1's tiles have landed for every wave, and every wave has read step e's
-          load(e + 2);
-          read_b(e + 1, 0), fa[0] = frag(e + 1, 0, wm * G::TM);
-        } else {
-          fa[(t + 1) & 1] = frag(e, (t + 1) / FA, wm * G::TM + 32 * ((t + 1) % FA));
-          if (t == FA - 1 - (FA > 1)) read_b(e, 1);
+      for (int t = 0; t < 2 * FA; ++t)  // part t: half t / FA, A's rows 32 (t % FA) on
+#pragma unroll
+        for (int i = 0; i < FB; ++i) {
+          if (t == 2 * FA - 1) {
+            if (i == 0) {
+              wait_vmem();
+              barrier_lds();  // step e + 1's tiles have landed for every wave, and every wave has read step e's
+              fa[0] = frag(e + 1, 0, wm * G::TM);
+            }
+            read_b(e + 1, 0, i);
+            load(e + 2, i * LOADS / FB, (i + 1) * LOADS / FB);
+          } else {
+            if (i == 0) fa[(t + 1) & 1] = frag(e, (t + 1) / FA, wm * G::TM + 32 * ((t + 1) % FA));
+            if (t == FA - 1 - (FA > 1)) read_b(e, 1, i);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          multiply(fa[t & 1], fb[t / FA][i], i, t % FA);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(fa[t & 1], fb[t / FA], t % FA);
-        __builtin_amdgcn_sched_barrier(0);
-      }
       scales(e - e0 + 1);  // (a chunk's first are read anew)
     }
   }
@@ -314,7 +322,7 @@ int go_rows(const kd_matmul8_args& g, hipStream_t st) {
 
 // Which tile: rounds of workgroups over the chip times a round's cost, in us, from
 // 8192^3 (a step of 128 columns) and 16384 x 4096 x 768 (start and end of a tile):
-//   256 x 256, one a CU:   466 us and 79 us -- 2.36 PFLOP/s in the large product
+//   256 x 256, one a CU:   450 us and 79 us
 //   128 x 128, two:        564        88
 //   64 x 64, four:         864       118, but 4.1 us against 5.7 and 12.5 where one round does (128 x 2048 x 768)
 // (columns of 64 instead of 128 a step: 16 TB/s instead of 25 from the L2, 528 us at best in the first;
@@ -331,7 +339,7 @@ int go(const kd_matmul8_args& g, hipStream_t st) {
     const int64_t tiles = (g.M + tile - 1) / tile * ((g.N + tile - 1) / tile);
     return double((tiles + at_once - 1) / at_once) * (ends + step * double(nb));
   };
-  const double large = cost(256, 256, 9.0, 1.82), mid = cost(128, 512, 4.3, 1.10), small = cost(64, 1024, 2.3, 0.84);
+  const double large = cost(256, 256, 9.0, 1.70), mid = cost(128, 512, 4.3, 1.10), small = cost(64, 1024, 2.3, 0.84);
   if constexpr (std::is_same_v<O, BF16> || std::is_same_v<O, F16>)  // (an fp32 tile of 256 x 256 does not fit the LDS on its way out)
     if (large < mid && large < small) return go_tiles<O, 256, 256, 2, 4, 1>(g, 4, st);
   if (mid < small) {

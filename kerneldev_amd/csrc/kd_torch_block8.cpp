@@ -67,6 +67,10 @@ void check_blocks(const Tensor& y, const Tensor& scale, int64_t cols, int64_t pe
                         aligned16(y),
                     what, ": values must lie in rows a multiple of 16 bytes apart, scales contiguous");
 }
+int32_t size32(int64_t n) {
+  TORCH_CHECK_VALUE(n < (int64_t(1) << 31), "sizes must be < 2^31, got ", n);
+  return int32_t(n);
+}
 // the blocks' values as the kernel reads them
 Tensor blocks_ready(const Tensor& y) {
   return y.dim() == 2 && y.stride(1) == 1 && y.stride(0) % 16 == 0 && y.stride(0) >= y.size(1) && aligned16(y) ? y : flat(y);
@@ -82,12 +86,12 @@ std::tuple<Tensor, Tensor> quant_rows8(at::TensorList xs) {
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == xs[0].size(0) && x.scalar_type() == xs[0].scalar_type(),
                       "the parts must be matrices of one type and one number of rows");
     keep.push_back(rows_ready(x));
-    a.x[a.n] = keep.back().data_ptr(), a.x_stride[a.n] = keep.back().stride(0), a.cols[a.n] = int32_t(x.size(1)), ++a.n;
+    a.x[a.n] = keep.back().data_ptr(), a.x_stride[a.n] = keep.back().stride(0), a.cols[a.n] = size32(x.size(1)), ++a.n;
     total += x.size(1);
   }
   const c10::DeviceGuard on(xs[0].device());
   a.dtype = dtype_code(xs[0].scalar_type(), true);
-  a.rows = xs[0].size(0), a.total = int32_t(total);
+  a.rows = xs[0].size(0), a.total = size32(total);
   Tensor y = bytes8(xs[0], a.rows, total), s = scales(xs[0], a.rows, blocks(total));
   if (a.rows == 0) return {y, s};
   a.y = u8(y), a.y_stride = y.stride(0), a.scale = u8(s);
@@ -105,12 +109,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> quant_weight8(at::TensorList ws, bool
     TORCH_CHECK_VALUE(w.dim() == 2 && w.size(1) == ws[0].size(1) && w.scalar_type() == ws[0].scalar_type(),
                       "the parts must be matrices of one type and one number of columns");
     keep.push_back(rows_ready(w));
-    a.w[a.n] = keep.back().data_ptr(), a.w_stride[a.n] = keep.back().stride(0), a.rows[a.n] = int32_t(w.size(0)), ++a.n;
+    a.w[a.n] = keep.back().data_ptr(), a.w_stride[a.n] = keep.back().stride(0), a.rows[a.n] = size32(w.size(0)), ++a.n;
     total += w.size(0);
   }
   const c10::DeviceGuard on(ws[0].device());
   const int64_t K = ws[0].size(1);
-  a.dtype = dtype_code(ws[0].scalar_type(), true), a.K = int32_t(K), a.total = int32_t(total);
+  a.dtype = dtype_code(ws[0].scalar_type(), true), a.K = size32(K), a.total = size32(total);
   Tensor y = bytes8(ws[0], total, K), s = scales(ws[0], blocks(total), blocks(K));
   Tensor yt = transpose ? bytes8(ws[0], K, total) : bytes8(ws[0], 0, 0);
   Tensor st = transpose ? scales(ws[0], blocks(K), blocks(total)) : scales(ws[0], 0, 0);
@@ -130,14 +134,13 @@ Tensor matmul8(const Tensor& a_in, const Tensor& a_scale, const Tensor& b_in, co
                     " and ", b.sizes());
   const int64_t M = a.size(0), N = b.size(0), K = a.size(1);
   check_blocks(a, as, K, 1, "a"), check_blocks(b, bs, K, 128, "b");
-  TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31) && K < (int64_t(1) << 31), "M, N and K must be < 2^31");
   kd_matmul8_args g{};
   g.dtype = dtype_code(out_type, true), g.fast = fast;
   Tensor out = fresh({M, N}, out_type, a);
   if (out.numel() == 0) return out;
   g.a = u8(a), g.b = u8(b), g.lda = a.stride(0), g.ldb = b.stride(0), g.a_scale = u8(as), g.b_scale = u8(bs);
   g.out = out.data_ptr(), g.ldo = N;
-  g.M = int32_t(M), g.N = int32_t(N), g.K = int32_t(K);
+  g.M = size32(M), g.N = size32(N), g.K = size32(K);
   check(kd_matmul8(&g, stream_of(out)), "kd_matmul8");
   return out;
 }
@@ -150,7 +153,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> norm8(const Tensor& x_in, const OptTe
   Tensor d, sum;
   kd_norm8_args a{};
   a.dtype = dtype_code(x.scalar_type(), false);
-  a.rows = x.size(0), a.D = int32_t(x.size(1)), a.eps = float(eps);
+  a.rows = x.size(0), a.D = size32(x.size(1)), a.eps = float(eps);
   if (delta) {
     on_one_gpu({&x, &*delta});
     TORCH_CHECK_VALUE(delta->sizes() == x.sizes() && delta->scalar_type() == x.scalar_type(),
@@ -184,7 +187,7 @@ Tensor norm8_bwd(const Tensor& g_in, const OptTensor& ds, const Tensor& y, const
   kd_norm8_bwd_args a{};
   a.dtype = dtype_code(dtype, false), a.g_dtype = dtype_code(g.scalar_type(), true);
   Tensor dx = fresh(g.sizes(), dtype, g);
-  a.rows = g.size(0), a.D = int32_t(g.size(1));
+  a.rows = g.size(0), a.D = size32(g.size(1));
   if (a.rows == 0) return dx;
   a.g = g.data_ptr(), a.ds = ds ? d.data_ptr() : nullptr, a.y = u8(y), a.y_stride = y.stride(0), a.scale = u8(scale);
   a.rstd = static_cast<const float*>(rstd.data_ptr()), a.dx = dx.data_ptr();
@@ -199,7 +202,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gate8(const Tensor& a
   const Tensor a = rows_ready(a_in), b = rows_ready(b_in);
   kd_gate8_args g{};
   g.dtype = dtype_code(a.scalar_type(), false);
-  g.rows = a.size(0), g.H = int32_t(a.size(1));
+  g.rows = a.size(0), g.H = size32(a.size(1));
   const int64_t kept = keep ? g.rows : 0, nb = blocks(g.H);
   Tensor y = bytes8(a, g.rows, g.H), ys = scales(a, g.rows, nb);
   Tensor a8 = bytes8(a, kept, g.H), as = scales(a, kept, nb), b8 = bytes8(a, kept, g.H), bs = scales(a, kept, nb);
@@ -222,7 +225,7 @@ std::tuple<Tensor, Tensor> gate8_bwd(const Tensor& dy_in, const Tensor& a8, cons
   Tensor da = fresh(dy.sizes(), dtype, dy), db = fresh(dy.sizes(), dtype, dy);
   kd_gate8_args g{};
   g.dtype = dtype_code(dtype, false), g.dy_dtype = dtype_code(dy.scalar_type(), true);
-  g.rows = dy.size(0), g.H = int32_t(dy.size(1));
+  g.rows = dy.size(0), g.H = size32(dy.size(1));
   if (g.rows == 0) return {da, db};
   g.dy = dy.data_ptr(), g.da = da.data_ptr(), g.db = db.data_ptr(), g.stride = a8.stride(0);
   g.a8 = u8(a8), g.a_scale = u8(as), g.b8 = u8(b8), g.b_scale = u8(bs);
@@ -244,17 +247,15 @@ Tensor weight_grad8(at::TensorList dys, const Tensor& x, const Tensor& x_scale, 
     const Tensor& dy = keep.back();
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == dy.size(0) && dy.scalar_type() == dys[0].scalar_type(),
                       "dy [M, N] of one type and x [M, K] expected, got ", dy.sizes(), " and ", x.sizes());
-    TORCH_CHECK_VALUE(dy.size(1) < (int64_t(1) << 31), "N must be < 2^31");
-    g.dy[g.n] = dy.data_ptr(), g.ldy[g.n] = dy.stride(0), g.cols[g.n] = int32_t(dy.size(1)), ++g.n;
+    g.dy[g.n] = dy.data_ptr(), g.ldy[g.n] = dy.stride(0), g.cols[g.n] = size32(dy.size(1)), ++g.n;
     N += dy.size(1);
   }
   check_blocks(x, x_scale, K, 1, "x");
   const int64_t M = x.size(0);
-  TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && N < (int64_t(1) << 31), "M and N must be < 2^31");
   g.dtype = dtype_code(dys[0].scalar_type(), false);
   if (M == 0) return at::zeros({N, K}, dys[0].options());
   Tensor dw = fresh({N, K}, dys[0].scalar_type(), x);
-  g.M = int32_t(M), g.N = int32_t(N), g.K = int32_t(K);
+  g.M = size32(M), g.N = size32(N), g.K = size32(K);
   g.ws_bytes = kd_weight_grad8_ws_bytes(g.M, g.N, g.K, g.dtype);
   check(g.ws_bytes < 0 ? KD_ERR_UNSUPPORTED : KD_OK, "kd_weight_grad8");
   const Tensor ws = fresh({g.ws_bytes}, at::kByte, x);

@@ -118,7 +118,8 @@ INVALID, UNSUPPORTED = _lib.KD_ERR_INVALID, _lib.KD_ERR_UNSUPPORTED
     ("kd_gate8", dict(H=60), UNSUPPORTED), ("kd_gate8", dict(a_stride=56), INVALID), ("kd_gate8", dict(b8=None), INVALID),
     ("kd_gate8", dict(y_scale=None), INVALID), ("kd_gate8_bwd", dict(a8=None), INVALID), ("kd_gate8_bwd", dict(da=P + 2), INVALID),
     ("kd_weight_grad8", dict(N=12), UNSUPPORTED), ("kd_weight_grad8", dict(N=24), INVALID), ("kd_weight_grad8", dict(n=0), INVALID),
-    ("kd_weight_grad8", dict(n=2, dy=[P, P], ldy=[16, 16], cols=[16, 16], N=32), INVALID), ("kd_weight_grad8", dict(M=0), INVALID), ("kd_weight_grad8", dict(ws_bytes=16), INVALID),
+    ("kd_weight_grad8", dict(n=2, dy=[P, P], ldy=[16, 16], cols=[16, 16], N=32), INVALID), ("kd_weight_grad8", dict(M=0), INVALID), ("kd_weight_grad8", dict(M=(1 << 31) - 1), UNSUPPORTED),
+    ("kd_weight_grad8", dict(ws_bytes=16), INVALID),
     ("kd_weight_grad8", dict(ldy=[12]), INVALID), ("kd_weight_grad8", dict(dy=[P + 8]), INVALID), ("kd_weight_grad8", dict(dtype=2), UNSUPPORTED), ("kd_weight_grad8", dict(x_scale=None), INVALID),
     ("kd_embed", dict(n=0), UNSUPPORTED), ("kd_embed", dict(vocab=0), UNSUPPORTED), ("kd_embed", dict(dim=0), UNSUPPORTED),
     ("kd_embed", dict(tokens=None), INVALID), ("kd_embed", dict(tokens_dtype=2), INVALID), ("kd_embed", dict(dtype=3), UNSUPPORTED),

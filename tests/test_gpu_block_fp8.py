@@ -516,6 +516,18 @@ def test_compiled(dev):
         torch.library.opcheck(op, args, test_utils="test_faketensor")  # (test_schema multiplies: no float8 there)
 
 
+@pytest.mark.parametrize("m,ns,k", [(20011, (2056,), 2064), (4096, (384, 128, 8), 256), (4100, (256, 264), 8), (33, (640,), 264)])
+def test_weight_grad_over_many_tokens(dev, m, ns, k):
+    """Pieces of more steps than scales are held at once, of exactly as many, and tiles past both edges.
+
+    The sums are fp32, in an order of the kernel's own: m products, each partial sum rounded once."""
+    dys = [_data((m, n), torch.bfloat16, dev, 3 + i) for i, n in enumerate(ns)]
+    x8, xs = torch.ops.kdattn.quant_rows8([_data((m, k), torch.bfloat16, dev, 1)])
+    dw = torch.ops.kdattn.weight_grad8(dys if len(dys) == 1 or ns[0] % 128 == 0 else [torch.cat(dys, 1)], x8, xs, k)
+    dy, kept = torch.cat(dys, 1).double(), _values(kd.BlockFp8(x8, xs))[:, :k]
+    _close(dw, dy.t() @ kept, m * 2.0 ** -23 * (dy.abs().t() @ kept.abs()))
+
+
 def test_offsets_past_32_bits(dev):
     """2^32 bytes of 8-bit rows, 2^33 of their source, 2^34 of a strided operand."""
     m, k = (1 << 21) + 3, 2064
