@@ -6,7 +6,11 @@
 // All are bound by memory.  A lane takes 8 values (16 bytes of a 16-bit
 // operand), so a block of 128 is a DPP row of 16 lanes and its maximum needs
 // four exchanges and no LDS; the values stay in registers between the maximum
-// and the rounding, so every operand is read once.
+// and the rounding, so every operand is read once.  At 16384 rows, bf16, with what
+// a pass has to read and write (a 64 MiB copy reaches 7.2 TB/s here, one of 1 GiB 5.1):
+//   rows of 2304 quantised     24 us  4.7 TB/s
+//   norm after addition, 768   17 us  5.0 TB/s, its backward 19 us  4.7 TB/s
+//   gate kept, 2048            47 us  5.0 TB/s, its backward 44 us  6.1 TB/s
 #include <algorithm>
 
 #include "kd_block8.h"
@@ -134,7 +138,7 @@ KD_DEV void turn4(const uint32_t (&r)[4], uint32_t (&c)[4]) {
 // A workgroup a block of 128 x 128, a thread 4 rows of 8 columns: the bytes go out
 // as they are and, turned over in registers, transposed.  Latency bounds it (a
 // model's weight is some hundred blocks): one round of loads, one exchange of the
-// maximum.
+// maximum (2304 x 768: 8.0 us, with 256 threads of 8 rows 10.5).
 template <class E>
 __global__ __launch_bounds__(512) void k_quant_weight(kd_weight8_args a, uint32_t kblocks, uint32_t nblocks) {
   __shared__ uint32_t s_max[8];
