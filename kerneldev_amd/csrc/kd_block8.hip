@@ -61,32 +61,42 @@ KD_DEV u32x2 quantise(const u32x4& v, uint32_t* byte) {
   return pack_finite(f, scale_value(*byte));
 }
 
+// Results of 16 MiB and more pass by the L2, which holds 32 (us, through it and past
+// it, sizes as above: rows 24.1 and 20.1, norm 18.3 and 15.5, its backward 16.2 and 14.8,
+// gate 45.0 and 42.6, its backward 48.6 and 46.1); smaller ones are read from it at once.
+constexpr int64_t PAST_BYTES = int64_t(1) << 24;
+template <class V>
+KD_DEV void put(V* p, const V& v, bool past) {
+  if (past) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
 // The lane's 8 values at column col of row `row` as part of their block, and
 // the block's scale byte by its first lane.  All lanes of a DPP row call it
 // together; those at or behind column `cols` hold zeros.
 KD_DEV void store_bytes(const u32x2& w, uint32_t byte, uint8_t* y, int64_t y_stride, uint8_t* scale, int64_t nb, int64_t row,
-                        int col, int cols) {
+                        int col, int cols, bool past) {
   if (col < (cols + 15) / 16 * 16)  // (the row's 16-byte words whole: zeros behind its end)
-    *reinterpret_cast<u32x2*>(y + row * y_stride + col) = w;
+    put(reinterpret_cast<u32x2*>(y + row * y_stride + col), w, past);
   if ((threadIdx.x & 15) == 0 && col < cols) scale[row * nb + col / QB] = uint8_t(byte);
 }
 KD_DEV void store_block(const float (&f)[8], uint8_t* y, int64_t y_stride, uint8_t* scale, int64_t nb, int64_t row,
-                        int col, int cols) {
+                        int col, int cols, bool past) {
   uint32_t b;
   const u32x2 w = quantise(f, &b);
-  store_bytes(w, b, y, y_stride, scale, nb, row, col, cols);
+  store_bytes(w, b, y, y_stride, scale, nb, row, col, cols, past);
 }
 template <class E>
 KD_DEV void store_block(const u32x4& v, uint8_t* y, int64_t y_stride, uint8_t* scale, int64_t nb, int64_t row, int col,
-                        int cols) {
+                        int cols, bool past) {
   uint32_t b;
   const u32x2 w = quantise<E>(v, &b);
-  store_bytes(w, b, y, y_stride, scale, nb, row, col, cols);
+  store_bytes(w, b, y, y_stride, scale, nb, row, col, cols, past);
 }
 
 // U blocks a DPP row of lanes, 16 apart: their loads go out together
 template <class E, int U>
-__global__ __launch_bounds__(256) void k_quant_rows(kd_rows8_args a, int64_t row0, uint32_t blocks, uint32_t nb) {
+__global__ __launch_bounds__(256) void k_quant_rows(kd_rows8_args a, int64_t row0, uint32_t blocks, uint32_t nb, bool past) {
   u32x4 v[U], hi[U];
   int64_t row[U];
   int col[U];
@@ -120,9 +130,9 @@ __global__ __launch_bounds__(256) void k_quant_rows(kd_rows8_args a, int64_t row
       float f[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(v[u][i]), f[4 + i] = __uint_as_float(hi[u][i]);
-      store_block(f, a.y, a.y_stride, a.scale, nb, row[u], col[u], a.total);
+      store_block(f, a.y, a.y_stride, a.scale, nb, row[u], col[u], a.total, past);
     } else {
-      store_block<E>(v[u], a.y, a.y_stride, a.scale, nb, row[u], col[u], a.total);
+      store_block<E>(v[u], a.y, a.y_stride, a.scale, nb, row[u], col[u], a.total, past);
     }
   }
 }
@@ -224,7 +234,7 @@ KD_DEV T row_sum(T x, T* s_part) {
 // value (rounded from an fp32 root, some ten of 10^7 were not).  Memory bounds it all
 // the same.
 template <class E, int NCH, int WPR>
-__global__ __launch_bounds__(256) void k_norm8(kd_norm8_args a, int64_t row0, int64_t end) {
+__global__ __launch_bounds__(256) void k_norm8(kd_norm8_args a, int64_t row0, int64_t end, bool past) {
   __shared__ double s_part[4];
   const int lane = threadIdx.x & (64 * WPR - 1);
   const int64_t at = row0 + int64_t(blockIdx.x) * (4 / WPR) + threadIdx.x / (64 * WPR);
@@ -248,7 +258,7 @@ __global__ __launch_bounds__(256) void k_norm8(kd_norm8_args a, int64_t row0, in
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[c][i] += g[i];
       const u32x4 s = pack8<E>(f[c]);
-      if (live && w < words) static_cast<u32x4*>(a.sum)[row * words + w] = s;
+      if (live && w < words) put(static_cast<u32x4*>(a.sum) + row * words + w, s, past);
       unpack8<E>(s, f[c]);
     }
   }
@@ -266,13 +276,13 @@ __global__ __launch_bounds__(256) void k_norm8(kd_norm8_args a, int64_t row0, in
   for (int c = 0; c < NCH; ++c) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[c][i] = __builtin_fmaf(f[c][i], r, f[c][i] * rest);
-    if (live) store_block(f[c], a.y, a.y_stride, a.scale, nb, row, (lane + 64 * WPR * c) * 8, a.D);
+    if (live) store_block(f[c], a.y, a.y_stride, a.scale, nb, row, (lane + 64 * WPR * c) * 8, a.D, past);
   }
 }
 
 // dx = ds + r (g - y mean(g y)), y from its 8 bits; g in E or (EG) fp32
 template <class E, class EG, int NCH, int WPR>
-__global__ __launch_bounds__(256) void k_norm8_bwd(kd_norm8_bwd_args a, int64_t row0, int64_t end) {
+__global__ __launch_bounds__(256) void k_norm8_bwd(kd_norm8_bwd_args a, int64_t row0, int64_t end, bool past) {
   __shared__ float s_part[4];
   const int lane = threadIdx.x & (64 * WPR - 1);
   const int64_t at = row0 + int64_t(blockIdx.x) * (4 / WPR) + threadIdx.x / (64 * WPR);
@@ -304,7 +314,7 @@ __global__ __launch_bounds__(256) void k_norm8_bwd(kd_norm8_bwd_args a, int64_t 
     if (a.ds != nullptr) unpack8<E>(w < words ? (static_cast<const u32x4*>(a.ds) + row * words)[w] : u32x4{}, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) g[c][i] = s[i] + r * (g[c][i] - f[c][i] * m);
-    if (w < words) static_cast<u32x4*>(a.dx)[row * words + w] = pack8<E>(g[c]);
+    if (w < words) put(static_cast<u32x4*>(a.dx) + row * words + w, pack8<E>(g[c]), past);
   }
 }
 
@@ -313,7 +323,7 @@ KD_DEV float sigmoid8(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(x 
 
 // y = silu(a) b, and a and b themselves, in 8 bits
 template <class E>
-__global__ __launch_bounds__(256) void k_gate8(kd_gate8_args g, int64_t row0, uint32_t blocks, uint32_t nb) {
+__global__ __launch_bounds__(256) void k_gate8(kd_gate8_args g, int64_t row0, uint32_t blocks, uint32_t nb, bool past) {
   const uint32_t blk = blockIdx.x * 16u + (threadIdx.x >> 4);
   const uint32_t r = blk / nb, kb = blk - r * nb;
   const int64_t row = row0 + r;
@@ -328,16 +338,16 @@ __global__ __launch_bounds__(256) void k_gate8(kd_gate8_args g, int64_t row0, ui
   unpack8<E>(va, a), unpack8<E>(vb, b);
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = a[i] * sigmoid8(a[i]) * b[i];
-  store_block(y, g.y8, g.stride, g.y_scale, nb, row, col, g.H);
+  store_block(y, g.y8, g.stride, g.y_scale, nb, row, col, g.H, past);
   if (g.a8 == nullptr) return;
-  store_block<E>(va, g.a8, g.stride, g.a_scale, nb, row, col, g.H);
-  store_block<E>(vb, g.b8, g.stride, g.b_scale, nb, row, col, g.H);
+  store_block<E>(va, g.a8, g.stride, g.a_scale, nb, row, col, g.H, past);
+  store_block<E>(vb, g.b8, g.stride, g.b_scale, nb, row, col, g.H, past);
 }
 
 // da = dy b s (1 + a (1 - s)), db = dy a s, s = sigmoid(a); a and b from their 8 bits
 template <class E, class EG>
 __global__ __launch_bounds__(256) void k_gate8_bwd(kd_gate8_args g, int64_t row0, uint32_t words_all, uint32_t words,
-                                                   uint32_t nb) {
+                                                   uint32_t nb, bool past) {
   const uint32_t i = blockIdx.x * 256u + threadIdx.x;
   if (i >= words_all) return;
   const uint32_t r = i / words, w = i - r * words;
@@ -353,8 +363,8 @@ __global__ __launch_bounds__(256) void k_gate8_bwd(kd_gate8_args g, int64_t row0
     da[k] = d[k] * v * s * (1.f + u * (1.f - s));
     db[k] = d[k] * (u * s);
   }
-  *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(g.da) + at) = pack8<E>(da);
-  *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(g.db) + at) = pack8<E>(db);
+  put(reinterpret_cast<u32x4*>(static_cast<uint16_t*>(g.da) + at), pack8<E>(da), past);
+  put(reinterpret_cast<u32x4*>(static_cast<uint16_t*>(g.db) + at), pack8<E>(db), past);
 }
 
 template <class F>
@@ -390,11 +400,12 @@ void norm_variant(int D, G go) {  // waves a row and words a lane
 // 8.3, but 2048 x 768 2.6 and 2.9, 633 x 1000 2.3 and 2.7; four 27.3, 9.1, 3.9, 3.9.  fp32: 16384 x 768 11.4 and 11.7.
 int launch_quant_rows(const kd_rows8_args& a, hipStream_t st) {
   const uint32_t nb = uint32_t((a.total + QB - 1) / QB);
+  const bool past = a.rows * a.total >= PAST_BYTES;
   auto go = [&](auto e, auto u) {
     constexpr int U = decltype(u)::value;
     in_launches(a.rows, 16 * int64_t(nb), [&](int64_t r, int64_t n) {
       const uint32_t blocks = uint32_t(n) * nb;
-      hipLaunchKernelGGL((k_quant_rows<decltype(e), U>), dim3((blocks + 16 * U - 1) / (16 * U)), dim3(256), 0, st, a, r, blocks, nb);
+      hipLaunchKernelGGL((k_quant_rows<decltype(e), U>), dim3((blocks + 16 * U - 1) / (16 * U)), dim3(256), 0, st, a, r, blocks, nb, past);
     });
   };
   using one = std::integral_constant<int, 1>;
@@ -425,7 +436,7 @@ int launch_norm8(const kd_norm8_args& a, hipStream_t st) {
       constexpr int W = decltype(wpr)::value;
       in_launches(a.rows, 64 * W, [&](int64_t r, int64_t n) {
         hipLaunchKernelGGL((k_norm8<E, decltype(nch)::value, W>), dim3(unsigned((n * W + 3) / 4)), dim3(256), 0, st, a, r,
-                           r + n);
+                           r + n, a.rows * a.D * (a.delta != nullptr ? 3 : 1) >= PAST_BYTES);
       });
     });
   });
@@ -438,7 +449,7 @@ int launch_norm8_bwd(const kd_norm8_bwd_args& a, hipStream_t st) {
       constexpr int W = decltype(wpr)::value;
       in_launches(a.rows, 64 * W, [&](int64_t r, int64_t n) {
         auto k = a.g_dtype == KD_F32 ? k_norm8_bwd<E, F32, decltype(nch)::value, W> : k_norm8_bwd<E, E, decltype(nch)::value, W>;
-        hipLaunchKernelGGL(k, dim3(unsigned((n * W + 3) / 4)), dim3(256), 0, st, a, r, r + n);
+        hipLaunchKernelGGL(k, dim3(unsigned((n * W + 3) / 4)), dim3(256), 0, st, a, r, r + n, 2 * a.rows * a.D >= PAST_BYTES);
       });
     });
   });
@@ -449,7 +460,8 @@ int launch_gate8(const kd_gate8_args& a, hipStream_t st) {
   return by_type(a.dtype, [&](auto e) {
     in_launches(a.rows, 16 * int64_t(nb), [&](int64_t r, int64_t n) {
       const uint32_t blocks = uint32_t(n) * nb;
-      hipLaunchKernelGGL(k_gate8<decltype(e)>, dim3((blocks + 15) / 16), dim3(256), 0, st, a, r, blocks, nb);
+      hipLaunchKernelGGL(k_gate8<decltype(e)>, dim3((blocks + 15) / 16), dim3(256), 0, st, a, r, blocks, nb,
+                         a.rows * a.H * (a.a8 != nullptr ? 3 : 1) >= PAST_BYTES);
     });
   });
 }
@@ -460,7 +472,7 @@ int launch_gate8_bwd(const kd_gate8_args& a, hipStream_t st) {
     in_launches(a.rows, int64_t(words), [&](int64_t r, int64_t n) {
       const uint32_t all = uint32_t(n) * words;
       auto k = a.dy_dtype == KD_F32 ? k_gate8_bwd<decltype(e), F32> : k_gate8_bwd<decltype(e), decltype(e)>;
-      hipLaunchKernelGGL(k, dim3((all + 255) / 256), dim3(256), 0, st, a, r, all, words, nb);
+      hipLaunchKernelGGL(k, dim3((all + 255) / 256), dim3(256), 0, st, a, r, all, words, nb, 4 * a.rows * a.H >= PAST_BYTES);
     });
   });
 }
