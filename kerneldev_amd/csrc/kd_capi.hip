@@ -287,7 +287,7 @@ int kd_quant_weight8(const kd_weight8_args* a, void* stream) {
     total += a->rows[i];
   }
   if (total != a->total) return fail(KD_ERR_INVALID, "total must be the sum of rows");
-  if (up(total, 128) / 128 * (up(a->K, 128) / 128) >= (1 << 24)) return fail(KD_ERR_UNSUPPORTED, "too many blocks");
+  if (up(total, 128) / 128 * (up(a->K, 128) / 128) >= (1 << 23)) return fail(KD_ERR_UNSUPPORTED, "too many blocks");
   if ((r = check_rows8(a->y, a->y_stride, a->K))) return r;
   if (a->scale == nullptr || (a->yt == nullptr) != (a->scale_t == nullptr))
     return fail(KD_ERR_INVALID, "scale is required, and yt and scale_t go together");
@@ -308,7 +308,7 @@ int kd_matmul8(const kd_matmul8_args* a, void* stream) {
   if ((r = check_rows8(a->a, a->lda, a->K)) || (r = check_rows8(a->b, a->ldb, a->K))) return r;
   if (a->a_scale == nullptr || a->b_scale == nullptr) return fail(KD_ERR_INVALID, "a_scale and b_scale are required");
   if (a->out == nullptr || !aligned16(a->out) || a->ldo < a->N) return fail(KD_ERR_INVALID, "out must be given, 16-byte aligned, its rows N apart or more");
-  if (up(a->M, 128) / 128 * (up(a->N, 128) / 128) >= (1 << 24)) return fail(KD_ERR_UNSUPPORTED, "M * N exceeds the grid limit");
+  if (up(a->M, 128) / 128 * (up(a->N, 128) / 128) >= (1 << 23)) return fail(KD_ERR_UNSUPPORTED, "M * N exceeds the grid limit");
   r = kd::launch_matmul8(*a, as_stream(stream));
   return r ? fail(r, "kernel launch failed (8-bit product)") : KD_OK;
 }

@@ -250,11 +250,12 @@ struct Runs {
   float* part;  // [chunk][2][dim]: the run that comes in from the chunk before; the one that starts here and goes on
   int64_t chunks;
   int tiles;
+  int64_t first;  // unit (a chunk's tile of columns) of this launch
 };
 
 template <class E, int V>
 __global__ __launch_bounds__(256) void k_embed_runs(kd_embed_args a, Runs s) {
-  const int64_t unit = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t unit = s.first + int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (unit >= s.chunks * s.tiles) return;
   const int64_t chunk = unit / s.tiles;
   const int lane = threadIdx.x & 63, col = int(unit - chunk * s.tiles) * 64 * V + lane * V;
@@ -323,8 +324,8 @@ __global__ __launch_bounds__(256) void k_embed_runs(kd_embed_args a, Runs s) {
 template <class E, int V>
 __global__ __launch_bounds__(64 * JOIN_W) void k_embed_join(kd_embed_args a, Runs s) {
   __shared__ float s_sum[JOIN_W][64 * V];
-  const int64_t chunk = blockIdx.x / s.tiles;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = int(blockIdx.x - chunk * s.tiles) * 64 * V + lane * V;
+  const int64_t unit = s.first + blockIdx.x, chunk = unit / s.tiles;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = int(unit - chunk * s.tiles) * 64 * V + lane * V;
   const int64_t i0 = chunk * CHUNK, i1 = i0 + CHUNK;
   if (i1 >= a.n) return;  // (all uniform up to the sums)
   const uint32_t run = s.keys[i1 - 1];
@@ -513,7 +514,8 @@ int launch_embed_grad(const kd_embed_args& a, uint8_t* ws, hipStream_t st) {
   if (a.n <= SMALL_N)
     return by_type(a.dtype, [&](auto e) {
       using E = decltype(e);
-      const int R = int(std::max<int64_t>(1, std::min<int64_t>(64, a.vocab / 1024)));
+      // (255 rows at most fit the list; a launch is less than 2^32 threads)
+      const int R = a.vocab >= (int64_t(1) << 29) ? 255 : int(std::max<int64_t>(1, std::min<int64_t>(64, a.vocab / 1024)));
       auto go = [&](auto v) {
         hipLaunchKernelGGL((k_embed_small<E, decltype(v)::value>), dim3(unsigned((a.vocab + R - 1) / R)), dim3(256), 0, st, a, R);
       };
@@ -541,10 +543,12 @@ int launch_embed_grad(const kd_embed_args& a, uint8_t* ws, hipStream_t st) {
     using E = decltype(e);
     auto go = [&](auto v) {
       constexpr int V = decltype(v)::value;
-      const Runs r{s.keys_out, s.idx_out, reinterpret_cast<float*>(ws + L.part), L.chunks, int((a.dim + 64 * V - 1) / (64 * V))};
-      const int64_t units = L.chunks * r.tiles;
-      hipLaunchKernelGGL((k_embed_runs<E, V>), dim3(unsigned((units + 3) / 4)), dim3(256), 0, st, a, r);
-      hipLaunchKernelGGL((k_embed_join<E, V>), dim3(unsigned(units)), dim3(64 * JOIN_W), 0, st, a, r);
+      Runs r{s.keys_out, s.idx_out, reinterpret_cast<float*>(ws + L.part), L.chunks, int((a.dim + 64 * V - 1) / (64 * V)), 0};
+      const int64_t units = L.chunks * r.tiles, most = 1 << 22;  // (a launch is less than 2^32 threads)
+      for (r.first = 0; r.first < units; r.first += 4 * most)
+        hipLaunchKernelGGL((k_embed_runs<E, V>), dim3(unsigned((std::min(4 * most, units - r.first) + 3) / 4)), dim3(256), 0, st, a, r);
+      for (r.first = 0; r.first < units; r.first += most)
+        hipLaunchKernelGGL((k_embed_join<E, V>), dim3(unsigned(std::min(most, units - r.first))), dim3(64 * JOIN_W), 0, st, a, r);
     };
     if (by_four(a, {a.dy, a.dw})) go(int_c<4>{});
     else go(int_c<1>{});

@@ -336,13 +336,15 @@ template <class O>
 int go(const kd_matmul8_args& g, hipStream_t st) {
   // Few rows, us, rows / tiles: 32 x 2048 x 768 3.2 / 4.3, 32 x 768 x 2048 5.1 / 6.5, 48 x 768 x 2048 6.9 / 6.5, 64 x 8192 x 8192
   // 53 / 46; fp32, whose tiles are slower, 64 x 768 x 2048 7.8 / 13.5
-  if (g.M <= 16) return go_rows<O, 1>(g, st);
-  if (g.M <= 32) return go_rows<O, 2>(g, st);
-  if (std::is_same_v<O, F32> && g.M <= 64) return go_rows<O, 4>(g, st);
+  // (a launch is less than 2^32 threads: up to 2^27 rows of B, or 2^23 tiles of 512 threads)
+  const bool rows = g.N < (1 << 27);
+  if (rows && g.M <= 16) return go_rows<O, 1>(g, st);
+  if (rows && g.M <= 32) return go_rows<O, 2>(g, st);
+  if (std::is_same_v<O, F32> && rows && g.M <= 64) return go_rows<O, 4>(g, st);
   const int64_t nb = (g.K + QB - 1) / QB;
   auto cost = [&](int64_t tile, int64_t at_once, double ends, double step) {
     const int64_t tiles = (g.M + tile - 1) / tile * ((g.N + tile - 1) / tile);
-    return double((tiles + at_once - 1) / at_once) * (ends + step * double(nb));
+    return tiles >= (1 << 23) ? 1e300 : double((tiles + at_once - 1) / at_once) * (ends + step * double(nb));
   };
   const double large = cost(256, 256, 9.0, 1.70), mid = cost(128, 512, 4.3, 1.10), small = cost(64, 1024, 2.3, 0.84);
   if constexpr (std::is_same_v<O, BF16> || std::is_same_v<O, F16>)  // (an fp32 tile of 256 x 256 does not fit the LDS on its way out)

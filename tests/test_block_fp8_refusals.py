@@ -110,6 +110,7 @@ INVALID, UNSUPPORTED = _lib.KD_ERR_INVALID, _lib.KD_ERR_UNSUPPORTED
     ("kd_matmul8", dict(K=24), UNSUPPORTED), ("kd_matmul8", dict(K=0), UNSUPPORTED), ("kd_matmul8", dict(M=0), INVALID),
     ("kd_matmul8", dict(lda=48), INVALID), ("kd_matmul8", dict(lda=72), INVALID), ("kd_matmul8", dict(a=P + 8), INVALID),
     ("kd_matmul8", dict(a_scale=None), INVALID), ("kd_matmul8", dict(ldo=15), INVALID), ("kd_matmul8", dict(dtype=4), UNSUPPORTED),
+    ("kd_matmul8", dict(M=1 << 30), UNSUPPORTED), ("kd_quant_weight8", dict(rows=[1 << 22], total=1 << 22, K=1 << 22, w_stride=[1 << 22], y_stride=1 << 22), UNSUPPORTED),
     ("kd_matmul8", dict(lda=1 << 24, ldb=1 << 24), INVALID), ("kd_matmul8", dict(M=(1 << 31) - 1, N=(1 << 31) - 1, ldo=1 << 31), UNSUPPORTED),
     ("kd_norm8", dict(D=60), UNSUPPORTED), ("kd_norm8", dict(D=8200), UNSUPPORTED), ("kd_norm8", dict(dtype=2), UNSUPPORTED),
     ("kd_norm8", dict(sum=None), INVALID), ("kd_norm8", dict(x=P + 2), INVALID), ("kd_norm8", dict(y_stride=48), INVALID),

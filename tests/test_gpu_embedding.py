@@ -154,3 +154,14 @@ def test_offsets_past_32_bits(dev):
                                                                             torch.cat([dy[:150], dy[250:]]).double())
     assert bool(((dw[-150:].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -16).all())
     assert torch.equal(dw[:100], dy[150:250]) and not dw[100:-150].any()
+
+
+def test_more_chunks_than_one_launch_takes(dev):
+    """Some 2^22 chunks of sorted positions; whole numbers, whose sums fp32 holds."""
+    n, vocab = (1 << 26) + (1 << 22) + 5, 300
+    g = torch.Generator(dev).manual_seed(1)
+    tokens = torch.randint(0, vocab, (n,), device=dev, generator=g, dtype=torch.int32)
+    dy = torch.randint(0, 3, (n, 1), device=dev, generator=g).float()
+    w = torch.zeros(vocab, 1, device=dev, requires_grad=True)
+    dw, = torch.autograd.grad(kd.embedding(tokens, w), w, dy)
+    assert torch.equal(dw[:, 0].double(), torch.bincount(tokens, weights=dy[:, 0].double(), minlength=vocab))
