@@ -8,9 +8,9 @@
 // four exchanges and no LDS; the values stay in registers between the maximum
 // and the rounding, so every operand is read once.  At 16384 rows, bf16, with what
 // a pass has to read and write (a 64 MiB copy reaches 7.2 TB/s here, one of 1 GiB 5.1):
-//   rows of 2304 quantised     24 us  4.7 TB/s
-//   norm after addition, 768   17 us  5.0 TB/s, its backward 19 us  4.7 TB/s
-//   gate kept, 2048            47 us  5.0 TB/s, its backward 44 us  6.1 TB/s
+//   rows of 2304 quantised     20 us  5.6 TB/s
+//   norm after addition, 768   16 us  5.5 TB/s, its backward 15 us  5.9 TB/s
+//   gate kept, 2048            43 us  5.5 TB/s, its backward 46 us  5.8 TB/s
 #include <algorithm>
 
 #include "kd_block8.h"
