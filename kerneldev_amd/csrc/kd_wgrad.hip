@@ -147,7 +147,8 @@ __global__ __launch_bounds__(256) void k_wgrad_sum(const float* __restrict__ par
 // step's one barrier.  dY and X's bytes are on their way two to three steps ahead.
 // What bounds it: of 4096^3's 140 us (0.98 PFLOP/s; the library's bf16 product of that
 // shape 131, a 128 x 128 tile with two workgroups a CU 183) the products alone take
-// 76, reads add 17, copies 17, the widening 9, the results and their sum 20.
+// 76, reads add 17, copies 17, the widening 9, the results and their sum 20.  Few
+// tokens pay for the large tile: 633 by 1000 x 528 17.5 us, 128 x 128 13.
 struct Wgrad8Args {
   const void* dy[4];
   int64_t ldy[4];
@@ -321,8 +322,8 @@ __global__ __launch_bounds__(256, 1) void k_wgrad8(Wgrad8Args w) {
     if (m == 0 || m == 2 || m == 3 || m == 4) bv[to][m == 0 ? 0 : m - 1] = read(tx, m == 0 ? 0 : m - 1, from_ks);
     else if (m < 8) av[to][m == 1 ? 0 : m - 4] = read(ty, m == 1 ? 0 : m - 4, from_ks);
   };
-  for (int i = 0; i < SLOTS - 1; ++i) load(i);
   fetch_scales(e0);
+  for (int i = 0; i < SLOTS - 1; ++i) load(i);
   wait_vmem_n<2 * (YL + XL)>();  // the first step's (copies of steps behind the piece fill with zeros, so counts hold)
   barrier_lds();
   take_x(0, 0);
@@ -364,16 +365,17 @@ __global__ __launch_bounds__(256, 1) void k_wgrad8(Wgrad8Args w) {
   }
   wait_vmem();  // (the copies behind the piece land before the LDS is given back)
   float* out = w.part + int64_t(piece) * w.N * w.K;
-  const bool whole = n0 + WT * wn + WT <= w.N && k0 + WT * wk + WT <= w.K;
 #pragma unroll
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const int k = k0 + WT * wk + 32 * b + c, n = n0 + WT * wn + 32 * a + 4 * hf;
+      const int k = k0 + WT * wk + 32 * b + c, nb = n0 + WT * wn + 32 * a, n = nb + 4 * hf;
       float* p = out + int64_t(n) * w.K + k;
-      if (whole) {
+      if (nb + 32 <= w.N) {  // (uniform: one test for the block's rows)
+        if (k < w.K) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[int64_t(8 * (r >> 2) + (r & 3)) * w.K] = acc[a][b][r];
+          for (int r = 0; r < 16; ++r) p[int64_t(8 * (r >> 2) + (r & 3)) * w.K] = acc[a][b][r];
+        }
       } else if (k < w.K) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
